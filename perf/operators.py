@@ -130,7 +130,8 @@ def _weights(g, shape, dtype, std=0.02):
 def _row_codes(x):
     """8-bit codes and float32 scale of every row of x."""
     x = x.float()
-    s = x.abs().amax(-1) / 127
+    m = x.abs().amax(-1)
+    s = m / torch.full_like(m, 127)  # by a Python number, torch multiplies with the rounded reciprocal
     q = torch.round(x / torch.where(s == 0, 1.0, s)[..., None]).clamp_(-127, 127)
     return q.to(torch.int8), s
 
