@@ -279,6 +279,62 @@ int gq_rtn_mxfp(const void* W, int w_dtype, int64_t rows, int64_t C, int mode, u
 int gq_dequantize(const uint8_t* q, const void* scales, const void* biases, int scale_dtype, int64_t rows,
                   int64_t C, int mode, int group_size, float* out, void* stream);
 
+/* RTN in 8-bit integers, symmetric, one float32 scale per row (no reference counterpart;
+ * the grid of gq_matmul_int8): s = max|x| / 127, q = clamp(rint(x / s), -127, 127), both as
+ * IEEE float32 operations; a row of zeros has s = 0. Rows with an Inf or NaN get a
+ * non-finite scale. X: [rows, C] of dtype, row stride ldx elements; q: int8 rows of stride
+ * ldq, columns [C, Cq) written as zeros (Cq: C rounded up to what the product wants);
+ * scales: fp32 [rows]. */
+int gq_rtn_int8(const void* X, int dtype, int64_t rows, int64_t C, int64_t ldx, int8_t* q, int64_t Cq, int64_t ldq,
+                float* scales, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Expert and 8-bit products (the forward of a layer; the reference runs them as one
+ * F.linear per expert, mlx_gptq/capture.py:192-207). Nothing here synchronizes or reads
+ * back: every call can be captured into a CUDA graph.
+ * ------------------------------------------------------------------------ */
+
+/* Slots of a top-k routing ordered by (expert, position, token). index: int32 or int64
+ * (index_bits) [T, k] expert of each token's positions; an index outside [0, E) drops the
+ * slot. tok: int32 [T * k], token of each ordered slot, -1 behind the last; slot: int32
+ * [T, k], where each (token, position) went, -1 if dropped; offsets: int64 [E + 1], first
+ * slot of every expert. E <= 1024, T * k < 2^31. */
+size_t gq_route_slots_workspace_size(int64_t T, int64_t k, int64_t E);
+int gq_route_slots(const void* index, int index_bits, int64_t T, int64_t k, int64_t E, int32_t* tok, int32_t* slot,
+                   int64_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[t] = sum over positions j of weights[t, j] * y[slot[t, j]], in position order in
+ * fp32, rounded once. y: [S, N] and out: [T, N] of dtype (GQ_BF16 / GQ_F16), row strides
+ * ldy / ldo elements; slot: int32 [T, k], entries outside [0, S) add nothing;
+ * weights: fp32 [T, k]. */
+int gq_combine_slots(const void* y, int dtype, int64_t S, int64_t ldy, const int32_t* slot, const float* weights,
+                     int64_t T, int64_t k, int64_t N, void* out, int64_t ldo, void* stream);
+
+/* Products grouped by expert with ragged sizes: Y[s] = X[rows[s]] W[e]^T for the rows
+ * offsets[e] <= s < offsets[e + 1] of expert e; glu: N = 2 I and
+ * Y[s, c] = silu(z[c]) * z[I + c], c < I. Sums (and SwiGLU) in fp32, rounded once.
+ * X: [n, K] of dtype (GQ_BF16 / GQ_F16), row stride ldx; rows: int32 [S], nullable (row s
+ * itself, n >= S); an index outside [0, n) stands for a row of zeros. offsets: int64
+ * [E + 1] on the device, non-decreasing from 0 (others are clamped to [0, S], never
+ * followed out of bounds); nullable with E = 1: all S rows. W: [E, N, K], strides ldw per
+ * channel and stride_w per expert. Y: [S, N] ([S, I] with glu), row stride ldy; rows from
+ * offsets[E] on are written as zeros with zero_behind != 0, else left as they were.
+ * K, ldx, ldw, stride_w multiples of 8, X and W 16-byte aligned; E <= 1024.
+ * engine: -1 chosen by sizes, 0 the few-rows kernel, 1 the tcgen05 kernel.
+ * status: optional device int32 (as in gq_prepare_hinv). */
+int gq_matmul_grouped(const void* X, int64_t n, int64_t ldx, const int32_t* rows, int64_t S, const int64_t* offsets,
+                      int64_t E, const void* W, int64_t N, int64_t K, int64_t ldw, int64_t stride_w, int dtype,
+                      int glu, void* Y, int64_t ldy, int zero_behind, int engine, int32_t* status, void* stream);
+
+/* The same for 8-bit codes: z = (Xq Wq^T, exact 32-bit sums) * xs[row] * ws[e, channel]
+ * (+ bias[channel], dense only: offsets NULL, no glu) in fp32, rounded once to out_dtype
+ * (GQ_BF16 / GQ_F16 / GQ_F32). xs: fp32 [n]; ws: fp32 [E, N]; K, ldx, ldw, stride_w
+ * multiples of 16, K <= 131071. */
+int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, const int32_t* rows, int64_t S,
+                   const int64_t* offsets, int64_t E, const int8_t* Wq, const float* ws, int64_t N, int64_t K,
+                   int64_t ldw, int64_t stride_w, const void* bias, int bias_dtype, int glu, void* Y, int out_dtype,
+                   int64_t ldy, int zero_behind, int engine, int32_t* status, void* stream);
+
 /* ------------------------------------------------------------------------
  * Packing (mlx_gptq/packing.py, mlx_gptq/artifacts.py)
  * ------------------------------------------------------------------------ */

@@ -70,6 +70,117 @@ __global__ void __launch_bounds__(256) rtn_mxfp_kernel(const void* __restrict__ 
 }
 
 // --------------------------------------------------------------------------
+// RTN in 8-bit integers, symmetric, one scale per row: s = max|x| / 127 and
+// q = clamp(rint(x / s), -127, 127), both IEEE float32 operations (ties to even), so the
+// codes do not depend on how the row is cut. A row of zeros (or one whose scale
+// underflows) has s = 0 and codes 0; a row with an Inf or NaN has a non-finite scale, which
+// every product with the row inherits.
+// HBM-bound: each row is read once and held in registers between its maximum and its
+// codes (rows beyond 8 vectors per thread are read again, from L2). TPR threads share a
+// row: a warp where a warp can hold one and there are rows for every SM, else the CTA.
+// --------------------------------------------------------------------------
+template <typename T, int V>
+__device__ __forceinline__ void load_row_vec(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32<T>(p[0]);
+  } else {
+    constexpr int PER = 16 / int(sizeof(T));  // elements per 16 bytes
+    T raw[V];
+#pragma unroll
+    for (int i = 0; i < V / PER; ++i)
+      *reinterpret_cast<uint4*>(raw + i * PER) = *reinterpret_cast<const uint4*>(p + i * PER);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32<T>(raw[i]);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[V], float s) {
+  int32_t c[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) c[i] = s > 0.0f ? max(-127, min(127, __float2int_rn(v[i] / s))) : 0;
+  if constexpr (V == 1) {
+    p[0] = int8_t(c[0]);
+  } else {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i >> 2] |= (uint32_t(c[i]) & 0xFFu) << (8 * (i & 3));
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+}
+
+template <typename T, int V, int TPR>
+__global__ void __launch_bounds__(256) rtn_int8_kernel(const T* __restrict__ X, int64_t rows, int64_t C, int64_t ldx,
+                                                       int8_t* __restrict__ q, int64_t Cq, int64_t ldq,
+                                                       float* __restrict__ scales) {
+  constexpr int NV = 8;  // vectors a thread holds
+  __shared__ uint32_t warp_max_bits[8];
+  const int sub = threadIdx.x % TPR;
+  const int64_t row = int64_t(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
+  const bool live = row < rows;
+  const T* x = X + (live ? row : 0) * ldx;
+  float v[NV][V];
+  uint32_t m = 0;  // max |x| as bits: ordered like the values, with Inf and NaN above them
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int64_t c = int64_t(sub + n * TPR) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[n][i] = 0.0f;
+    if (live && c < C) load_row_vec<T, V>(x + c, v[n]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(v[n][i]) & 0x7FFFFFFFu);
+  }
+  for (int64_t c = int64_t(sub + NV * TPR) * V; live && c < C; c += int64_t(TPR) * V) {
+    float w[V];
+    load_row_vec<T, V>(x + c, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(w[i]) & 0x7FFFFFFFu);
+  }
+  m = __reduce_max_sync(~0u, m);
+  if constexpr (TPR == 256) {
+    if ((threadIdx.x & 31) == 0) warp_max_bits[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, warp_max_bits[w]);
+  }
+  if (!live) return;
+  const float s = __uint_as_float(m) / 127.0f;
+  if (sub == 0) scales[row] = s;
+  int8_t* out = q + row * ldq;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int64_t c = int64_t(sub + n * TPR) * V;
+    if (c < Cq) store_codes<V>(out + c, v[n], s);  // columns from C on hold zeros
+  }
+  for (int64_t c = int64_t(sub + NV * TPR) * V; c < Cq; c += int64_t(TPR) * V) {
+    float w[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = 0.0f;
+    if (c < C) load_row_vec<T, V>(x + c, w);
+    store_codes<V>(out + c, w, s);
+  }
+}
+
+template <typename T>
+int rtn_int8(const void* X, int64_t rows, int64_t C, int64_t ldx, int8_t* q, int64_t Cq, int64_t ldq, float* scales,
+             cudaStream_t s) {
+  const T* x = reinterpret_cast<const T*>(X);
+  const bool wide = C % 8 == 0 && Cq % 8 == 0 && ldq % 8 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0 && aligned16(X) &&
+                    (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+  const bool by_warp = Cq <= (wide ? 2048 : 256) && rows >= 1184;  // 8 rows for each of 148 SMs
+  const unsigned grid = unsigned(by_warp ? (rows + 7) / 8 : rows);
+  if (wide && by_warp)
+    rtn_int8_kernel<T, 8, 32><<<grid, 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
+  else if (wide)
+    rtn_int8_kernel<T, 8, 256><<<grid, 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
+  else if (by_warp)
+    rtn_int8_kernel<T, 1, 32><<<grid, 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
+  else
+    rtn_int8_kernel<T, 1, 256><<<grid, 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
+  return check_launch("rtn_int8_kernel");
+}
+
+// --------------------------------------------------------------------------
 // dequantize_artifact
 // --------------------------------------------------------------------------
 __global__ void dequant_kernel(const uint8_t* __restrict__ q, const void* __restrict__ scales,
@@ -238,6 +349,19 @@ extern "C" int gq_rtn_mxfp(const void* W, int w_dtype, int64_t rows, int64_t C, 
   else
     rtn_mxfp_kernel<GQ_MXFP8><<<blocks_for(ng, 8), 256, 0, s>>>(W, w_dtype, ng, q, nullptr, scales, w_dq, wdq_dtype);
   return check_launch("rtn_mxfp_kernel");
+}
+
+extern "C" int gq_rtn_int8(const void* X, int dtype, int64_t rows, int64_t C, int64_t ldx, int8_t* q, int64_t Cq,
+                           int64_t ldq, float* scales, void* stream) {
+  GQ_REQUIRE(valid_dtype(dtype), "gq_rtn_int8: dtype");
+  GQ_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && C >= 1 && ldx >= C, "gq_rtn_int8: sizes");
+  GQ_REQUIRE(Cq >= C && ldq >= Cq, "gq_rtn_int8: %lld code columns for %lld", (long long)Cq, (long long)C);
+  if (rows == 0) return GQ_OK;
+  GQ_REQUIRE(X && q && scales, "gq_rtn_int8: null pointer");
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == GQ_BF16) return rtn_int8<__nv_bfloat16>(X, rows, C, ldx, q, Cq, ldq, scales, s);
+  if (dtype == GQ_F16) return rtn_int8<__half>(X, rows, C, ldx, q, Cq, ldq, scales, s);
+  return rtn_int8<float>(X, rows, C, ldx, q, Cq, ldq, scales, s);
 }
 
 extern "C" int gq_dequantize(const uint8_t* q, const void* scales, const void* biases, int scale_dtype, int64_t rows,

@@ -1,0 +1,83 @@
+// Products of activation rows with weights, grouped by expert (ragged) or dense:
+// what the few-rows kernel (gq_product_rows.cu) and the tcgen05 kernel
+// (gq_product_tc.cu) share.
+#pragma once
+
+#include "gq_common.cuh"
+
+namespace gq {
+namespace prod {
+
+// Element kinds of a product: both operands in the kind, sums in fp32 (s32 for S8, exact).
+enum Kind : int { BF16 = 0, F16 = 1, S8 = 2 };
+
+constexpr int64_t kMaxExperts = 1024;
+
+// Y[s] = op(X[rows[s]] W_e^T) for the rows s of expert e = [offsets[e], offsets[e + 1]).
+struct Args {
+  const uint8_t* X;        // [n_src, K]
+  int64_t n_src, ldx;      // ldx: bytes between rows, a multiple of 16
+  const int32_t* rows;     // [S] row of X per product row (nullable: row s itself)
+  const int64_t* offsets;  // [E + 1] on the device (nullable: one expert with all S rows)
+  int64_t E, S;
+  const uint8_t* W;        // [E, N, K]
+  int64_t N, K;            // output channels (2 * I with glu), contracted size in elements
+  int64_t ldw, stride_w;   // bytes between channels and between experts, multiples of 16
+  const float* xs;         // S8: [n_src] scale per row of X
+  const float* ws;         // S8: [E, N] scale per channel
+  const void* bias;        // [N], nullable (dense only)
+  int bias_dtype;
+  void* Y;                 // [S, N] (glu: [S, N / 2]) of out_dtype
+  int64_t ldy;             // elements
+  int out_dtype;
+  int zero_behind;         // rows behind the last expert's: 1 = written as zeros, 0 = left alone
+  int32_t* status;         // nullable
+};
+
+int launch_rows(const Args& a, Kind kind, bool glu, cudaStream_t s);
+int launch_tc(const Args& a, Kind kind, bool glu, cudaStream_t s);
+
+// Rows of expert e, whatever the offsets hold: 0 <= begin <= end <= S.
+__device__ __forceinline__ void segment(const Args& a, int64_t e, int64_t& begin, int64_t& end) {
+  if (!a.offsets) {
+    begin = 0, end = a.S;
+    return;
+  }
+  const int64_t b = a.offsets[e], f = a.offsets[e + 1];
+  begin = b < 0 ? 0 : (b > a.S ? a.S : b);
+  end = f < begin ? begin : (f > a.S ? a.S : f);
+}
+
+// First row behind the last expert's.
+__device__ __forceinline__ int64_t rows_end(const Args& a) {
+  if (!a.offsets) return a.S;
+  const int64_t f = a.offsets[a.E];
+  return f < 0 ? 0 : (f > a.S ? a.S : f);
+}
+
+// Row of X behind product row s, or -1 where there is none (its products are zero).
+__device__ __forceinline__ int64_t source_row(const Args& a, int64_t s) {
+  const int64_t r = a.rows ? int64_t(a.rows[s]) : s;
+  return r >= 0 && r < a.n_src ? r : -1;
+}
+
+__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
+  if (dtype == GQ_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == GQ_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+
+__device__ __forceinline__ void store_from_f32(void* p, int64_t i, float v, int dtype) {
+  if (dtype == GQ_BF16)
+    reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else if (dtype == GQ_F16)
+    reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+  else
+    reinterpret_cast<float*>(p)[i] = v;
+}
+
+// silu(g) * u in fp32: the one rounding to the output's type comes after it.
+__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+}  // namespace prod
+}  // namespace gq

@@ -9,6 +9,8 @@ tensors.
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib as L
@@ -105,6 +107,37 @@ def rtn_quantize_mxfp(W: torch.Tensor, mode: str):
     L.check(L.lib().gq_rtn_mxfp(L.ptr(Wc), _dtype_code(Wc.dtype), rows, C, L.MODE_CODE[mode], L.ptr(q), None,
                                 L.ptr(s), L.ptr(dq), L.GQ_F32, L.stream_ptr(dev)), "rtn_quantize_mxfp")
     return q, s, None, dq
+
+
+def _int8_codes(rows: torch.Tensor, columns: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """int8 codes [n, columns] (zeros from column C on) and float32 scales [n] of rows [n, C]."""
+    n, C = rows.shape
+    if (C > 1 and rows.stride(1) != 1) or (n > 1 and rows.stride(0) < C):
+        rows = rows.contiguous()
+    dev = rows.device
+    q = torch.empty(n, columns, dtype=torch.int8, device=dev)
+    s = torch.empty(n, dtype=torch.float32, device=dev)
+    with contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
+        L.check(L.lib().gq_rtn_int8(L.ptr(rows), _dtype_code(rows.dtype), n, C, rows.stride(0) if n > 1 else C,
+                                    L.ptr(q), columns, columns, L.ptr(s), L.stream_ptr(dev)), "rtn_quantize_int8")
+    return q, s
+
+
+@torch.no_grad()
+def rtn_quantize_int8(W: torch.Tensor):
+    """RTN in 8-bit integers, symmetric, one scale per row (no reference counterpart): the
+    grid of products.matmul_int8, for weights (a row is an output channel) and for
+    activations (a row is a token). W [..., cols] in bf16, f16 or f32.
+
+    Returns (q int8 [..., cols], scales float32 [...]) with s = max|w| / 127 and
+    q = clamp(rint(w / s), -127, 127), IEEE float32 operations; a row of zeros has s = 0, a
+    row with an Inf or NaN a non-finite scale (which its products inherit)."""
+    L.require_cuda(W)
+    if W.dim() == 0 or W.shape[-1] == 0:
+        raise ValueError("rtn_quantize_int8 needs rows of at least one column")
+    _dtype_code(W.dtype)
+    q, s = _int8_codes(W.reshape(-1, W.shape[-1]), W.shape[-1])
+    return q.reshape(W.shape), s.reshape(W.shape[:-1])
 
 
 @torch.no_grad()

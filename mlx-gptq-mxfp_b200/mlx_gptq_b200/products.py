@@ -1,0 +1,320 @@
+"""Products of a layer's forward on the GPU: expert products and 8-bit products.
+
+The forward of a calibrated layer multiplies activation rows with weights; the
+reference does so with one ``F.linear`` per expert (mlx_gptq/capture.py:192-207).
+Here:
+
+* ``route_slots`` / ``combine_slots``: the order of a top-k routing's slots by expert,
+  and the weighted sum of the slots' rows per token;
+* ``matmul_grouped``: rows of every expert times that expert's weights, ragged sizes,
+  rows optionally taken through a row list, SwiGLU optionally applied, one launch;
+* ``expert_mlp``: the expert MLP of a routed batch from the three above;
+* ``matmul_int8`` / ``matmul_grouped_int8`` / ``linear_int8``: the same products on 8-bit
+  codes with one scale per row and one per channel (codes from
+  ``grid.rtn_quantize_int8``).
+
+All run on the tensors' CUDA device and its current stream and never wait for the
+device, so they can be captured into a CUDA graph (after one ordinary call per device).
+They have no backward: with gradients enabled, inputs that require them are refused.
+"""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _lib as L
+
+MAX_EXPERTS = 1024
+ENGINES = {None: -1, "rows": 0, "tcgen05": 1}
+
+
+def _forward_only(what: str, *tensors) -> torch.device:
+    """The tensors' common CUDA device; refuses a call that autograd would have to follow."""
+    dev = L.require_cuda(*tensors)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
+    return dev
+
+
+def _on(dev: torch.device):
+    """Launches go to `dev`, whatever device is current."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _status(dev: torch.device) -> torch.Tensor:
+    """The device's status word; its first use allocates it, which must not be captured."""
+    if torch.cuda.is_current_stream_capturing() and dev.index not in L._status_words:
+        raise RuntimeError("make one call on this device before capturing a CUDA graph")
+    return L.status_word(dev)
+
+
+def _engine(engine) -> int:
+    if engine not in ENGINES:
+        raise ValueError(f"unknown engine {engine!r} (one of {list(ENGINES)})")
+    return ENGINES[engine]
+
+
+def _operand(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """(operand, row stride, expert stride) as the kernels read it: whole rows, every row
+    16-byte aligned. Anything else (an odd contracted size, a transposed view) is copied,
+    padded with zeros to a multiple of 16 bytes."""
+    m = 16 // t.element_size()
+    K = t.shape[-1]
+
+    def strides(x):
+        ld = x.stride(-2) if x.shape[-2] > 1 else x.shape[-1]
+        return ld, (x.stride(0) if x.dim() == 3 and x.shape[0] > 1 else x.shape[-2] * ld)
+
+    ld, outer = strides(t)
+    if (K % m or (K > 1 and t.stride(-1) != 1) or ld < K or ld % m or outer < K or outer % m or t.data_ptr() % 16):
+        p = torch.zeros(*t.shape[:-1], -(-K // m) * m, dtype=t.dtype, device=t.device)
+        p[..., :K] = t
+        t = p
+        ld, outer = strides(t)
+    return t, ld, outer
+
+
+def _row_list(rows: torch.Tensor | None, n: int) -> torch.Tensor | None:
+    if rows is None:
+        return None
+    if rows.dim() != 1 or rows.dtype not in (torch.int32, torch.int64):
+        raise ValueError("rows must be a 1-D int32 or int64 tensor")
+    if rows.dtype == torch.int64:
+        rows = rows.clamp(-1, n)  # an index outside stays outside in 32 bits
+    return rows.to(torch.int32).contiguous()
+
+
+def _offsets(offsets: torch.Tensor, E: int, dev: torch.device) -> torch.Tensor:
+    if offsets.dim() != 1 or offsets.shape[0] != E + 1 or offsets.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"offsets must be int64 [{E + 1}] (experts + 1)")
+    return offsets.to(dev, torch.int64).contiguous()
+
+
+def _output(out, shape, dtype, dev, name="out") -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != dev:
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on {dev}")
+    if (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1]):
+        raise ValueError(f"{name} must have whole rows that do not overlap")
+    return out
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _channels(w: torch.Tensor, glu: bool) -> int:
+    if glu and w.shape[-2] % 2:
+        raise ValueError(f"glu needs an even number of channels (gate, then up), not {w.shape[-2]}")
+    return w.shape[-2] // 2 if glu else w.shape[-2]
+
+
+def _check_pair(x: torch.Tensor, w: torch.Tensor, w_dims: int) -> None:
+    if x.dim() != 2 or w.dim() != w_dims or x.shape[1] != w.shape[-1]:
+        raise ValueError(f"shapes: rows [n, K] {list(x.shape)}, weights {'[E, N, K]' if w_dims == 3 else '[N, K]'} "
+                         f"{list(w.shape)}")
+    if 0 in w.shape:
+        raise ValueError(f"weights {list(w.shape)} are empty")
+    if w_dims == 3 and w.shape[0] > MAX_EXPERTS:
+        raise ValueError(f"{w.shape[0]} experts, at most {MAX_EXPERTS}")
+
+
+def route_slots(top_k_index: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Slots of a routing ordered by (expert, top-k position, token): the row order of the
+    reference's per-expert torch.where (see experts.py), without reading counts back.
+
+    top_k_index: int32 or int64 [T, k]; an index outside [0, num_experts) drops its slot.
+    Returns (tok, slot, offsets): tok int32 [T * k], the token of every ordered slot (-1
+    behind the last); slot int32 [T, k], where each went (-1 if dropped); offsets int64
+    [num_experts + 1], the first slot of every expert."""
+    dev = L.require_cuda(top_k_index)
+    if top_k_index.dim() != 2 or top_k_index.dtype not in (torch.int32, torch.int64) or top_k_index.shape[1] == 0:
+        raise ValueError("top_k_index must be int32 or int64 [tokens, k]")
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ValueError(f"{num_experts} experts, 1 to {MAX_EXPERTS}")
+    T, k = top_k_index.shape
+    idx = top_k_index.contiguous()
+    tok = torch.empty(T * k, dtype=torch.int32, device=dev)
+    slot = torch.empty(T, k, dtype=torch.int32, device=dev)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int64, device=dev)
+    lib = L.lib()
+    ws_bytes = lib.gq_route_slots_workspace_size(T, k, num_experts)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with _on(dev):
+        L.check(lib.gq_route_slots(L.ptr(idx), 8 * idx.element_size(), T, k, num_experts, L.ptr(tok), L.ptr(slot),
+                                   L.ptr(offsets), L.ptr(ws), ws_bytes, L.stream_ptr(dev)), "route_slots")
+    return tok, slot, offsets
+
+
+def combine_slots(y: torch.Tensor, slot: torch.Tensor, weights: torch.Tensor,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[t] = sum over positions j of weights[t, j] * y[slot[t, j]], in position order in
+    float32, rounded once to y's type. y: bf16 or f16 [S, N]; slot: int32 [T, k] from
+    route_slots (entries outside [0, S) add nothing); weights: float [T, k]."""
+    dev = _forward_only("combine_slots", y, slot, weights, out)
+    if y.dim() != 2 or y.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("y must be bf16 or f16 [slots, channels]")
+    if slot.dim() != 2 or slot.dtype != torch.int32 or weights.shape != slot.shape or 0 in slot.shape[1:]:
+        raise ValueError("slot must be int32 [tokens, k] and weights [tokens, k]")
+    if not weights.is_floating_point():
+        raise ValueError("weights must be floating point")
+    (T, k), (S, N) = slot.shape, y.shape
+    if (N > 1 and y.stride(1) != 1) or (S > 1 and y.stride(0) < N):
+        y = y.contiguous()
+    out = _output(out, (T, N), y.dtype, dev)
+    if T == 0 or N == 0:
+        return out
+    sl, w = slot.contiguous(), weights.to(torch.float32).contiguous()
+    with _on(dev):
+        L.check(L.lib().gq_combine_slots(L.ptr(y), L.DTYPE_CODE[y.dtype], S, _ld(y), L.ptr(sl), L.ptr(w), T, k, N,
+                                         L.ptr(out), _ld(out), L.stream_ptr(dev)), "combine_slots")
+    return out
+
+
+def matmul_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows: torch.Tensor | None = None,
+                   glu: bool = False, out: torch.Tensor | None = None, engine: str | None = None) -> torch.Tensor:
+    """y[s] = x[rows[s]] @ w[e].T for the rows offsets[e] <= s < offsets[e + 1] of expert e.
+
+    x: bf16 or f16 [n, K]; w: the same type [E, N, K]; offsets: int64 [E + 1],
+    non-decreasing from 0; rows: int32 / int64 [S] (default: row s itself; an index outside
+    [0, n) is a row of zeros). glu: the channels are [gate; up] and
+    y = silu(x gate.T) * (x up.T), [S, N / 2]. Sums and SwiGLU in float32, rounded once.
+    Rows behind the last expert's are zeros, or left as they were in a given `out` (which
+    must not overlap the inputs). engine: None picks by sizes, "rows" reads the weights
+    once per few rows, "tcgen05" is the tensor-core kernel."""
+    dev = _forward_only("matmul_grouped", x, w, rows, out)
+    _check_pair(x, w, 3)
+    if x.dtype != w.dtype or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"rows and weights must both be bf16 or f16, not {x.dtype} and {w.dtype}")
+    E, N, _ = w.shape
+    off = _offsets(offsets, E, dev)
+    idx = _row_list(rows, x.shape[0])
+    S = x.shape[0] if idx is None else idx.shape[0]
+    y = _output(out, (S, _channels(w, glu)), x.dtype, dev)
+    if S == 0:
+        return y
+    if x.shape[0] == 0:
+        raise ValueError("rows of an empty x")
+    xo, ldx, _ = _operand(x)
+    wo, ldw, stride_w = _operand(w)
+    with _on(dev):
+        L.check(L.lib().gq_matmul_grouped(L.ptr(xo), xo.shape[0], ldx, L.ptr(idx), S, L.ptr(off), E, L.ptr(wo), N,
+                                          wo.shape[-1], ldw, stride_w, L.DTYPE_CODE[x.dtype], int(glu), L.ptr(y),
+                                          _ld(y), int(out is None), _engine(engine), L.ptr(_status(dev)),
+                                          L.stream_ptr(dev)), "matmul_grouped")
+    return y
+
+
+def expert_mlp(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.Tensor, gate_up: torch.Tensor,
+               down: torch.Tensor, acts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The expert MLP of a routed batch: out[t] = sum_j weights[t, j] * down_e(silu(gate_e x_t) * up_e x_t)
+    with e = top_k_index[t, j].
+
+    x: bf16 or f16 [T, C]; top_k_index: int32 / int64 [T, k] (an index outside [0, E) adds
+    nothing); top_k_weights: float [T, k]; gate_up: [E, 2 I, C] (gate channels, then up);
+    down: [E, C', I], in x's type. Products and sums are float32; the rows between the two
+    products and the rows before the sum are rounded to x's type. acts ([T * k, I]): where
+    the rows that feed down are written, in route_slots order (rows behind the last slot
+    are left alone). Returns [T, C']."""
+    dev = _forward_only("expert_mlp", x, top_k_index, top_k_weights, gate_up, down, acts, out)
+    _check_pair(x, gate_up, 3)
+    if down.dim() != 3 or down.shape[0] != gate_up.shape[0] or 2 * down.shape[2] != gate_up.shape[1]:
+        raise ValueError(f"shapes: gate_up [E, 2 I, C] {list(gate_up.shape)}, down [E, C', I] {list(down.shape)}")
+    if top_k_index.dim() != 2 or top_k_index.shape[0] != x.shape[0] or top_k_weights.shape != top_k_index.shape:
+        raise ValueError("top_k_index and top_k_weights must be [tokens, k]")
+    T, k = top_k_index.shape
+    I = down.shape[2]
+    acts = _output(acts, (T * k, I), x.dtype, dev, "acts")
+    out = _output(out, (T, down.shape[1]), x.dtype, dev)
+    if T == 0:
+        return out
+    tok, slot, offsets = route_slots(top_k_index, gate_up.shape[0])
+    matmul_grouped(x, gate_up, offsets, rows=tok, glu=True, out=acts)
+    y = torch.empty(T * k, down.shape[1], dtype=x.dtype, device=dev)
+    matmul_grouped(acts, down, offsets, out=y)
+    return combine_slots(y, slot, top_k_weights, out=out)
+
+
+def _scales(s: torch.Tensor, shape, name: str) -> torch.Tensor:
+    if s.dtype != torch.float32 or tuple(s.shape) != tuple(shape):
+        raise ValueError(f"{name} must be float32 {list(shape)}")
+    return s.contiguous()
+
+
+def _int8(xq, xs, wq, ws, offsets, rows, bias, glu, out_dtype, out, engine, what):
+    dev = _forward_only(what, xq, xs, wq, ws, rows, bias, out)
+    grouped = offsets is not None
+    _check_pair(xq, wq, 3 if grouped else 2)
+    if xq.dtype != torch.int8 or wq.dtype != torch.int8:
+        raise ValueError(f"codes must be int8, not {xq.dtype} and {wq.dtype}")
+    if out_dtype not in L.DTYPE_CODE:
+        raise ValueError(f"unsupported dtype {out_dtype}")
+    N, K = wq.shape[-2:]
+    E = wq.shape[0] if grouped else 1
+    if K > 131071:
+        raise ValueError(f"K = {K}: sums of 8-bit products fit 32 bits up to 131071")
+    xs = _scales(xs, xq.shape[:1], "xs")
+    ws = _scales(ws, wq.shape[:-1], "ws")
+    off = _offsets(offsets, E, dev) if grouped else None
+    idx = _row_list(rows, xq.shape[0])
+    S = xq.shape[0] if idx is None else idx.shape[0]
+    if bias is not None:
+        if bias.shape != (N,) or bias.dtype not in L.DTYPE_CODE:
+            raise ValueError(f"bias must be floating point [{N}]")
+        bias = bias.contiguous()
+    y = _output(out, (S, _channels(wq, glu)), out_dtype, dev)
+    if S == 0:
+        return y
+    if xq.shape[0] == 0:
+        raise ValueError("rows of an empty xq")
+    xo, ldx, _ = _operand(xq)
+    wo, ldw, stride_w = _operand(wq)
+    with _on(dev):
+        L.check(L.lib().gq_matmul_int8(L.ptr(xo), L.ptr(xs), xo.shape[0], ldx, L.ptr(idx), S, L.ptr(off), E,
+                                       L.ptr(wo), L.ptr(ws), N, wo.shape[-1], ldw, stride_w, L.ptr(bias),
+                                       0 if bias is None else L.DTYPE_CODE[bias.dtype], int(glu), L.ptr(y),
+                                       L.DTYPE_CODE[out_dtype], _ld(y), int(out is None), _engine(engine),
+                                       L.ptr(_status(dev)), L.stream_ptr(dev)), what)
+    return y
+
+
+def matmul_int8(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
+                bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                out: torch.Tensor | None = None, engine: str | None = None) -> torch.Tensor:
+    """y = (xq @ wq.T) * xs[:, None] * ws (+ bias): int8 codes xq [M, K] with a float32 scale
+    per row, wq [N, K] with one per channel. The integer sums are exact (K <= 131071);
+    scales and bias are applied in float32 and rounded once to out_dtype (bf16, f16, f32)."""
+    return _int8(xq, xs, wq, ws, None, None, bias, False, out_dtype, out, engine, "matmul_int8")
+
+
+def matmul_grouped_int8(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor,
+                        offsets: torch.Tensor, rows: torch.Tensor | None = None, glu: bool = False,
+                        out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+                        engine: str | None = None) -> torch.Tensor:
+    """matmul_grouped on int8 codes: xq [n, K] with scales xs [n], wq [E, N, K] with ws [E, N];
+    offsets, rows, glu and out as there (rows picks codes and scales alike)."""
+    if offsets is None:
+        raise ValueError("offsets must be int64 [experts + 1]")
+    return _int8(xq, xs, wq, ws, offsets, rows, None, glu, out_dtype, out, engine, "matmul_grouped_int8")
+
+
+def linear_int8(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias: torch.Tensor | None = None,
+                out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """A linear layer in 8 bits: the rows of x [..., K] (bf16, f16 or f32) quantized to int8
+    with one scale per row (grid.rtn_quantize_int8), times wq [N, K] / ws [N] quantized the
+    same way, + bias. Returns [..., N] in out_dtype (default: x's)."""
+    from .grid import _int8_codes
+
+    dev = _forward_only("linear_int8", x, wq, ws, bias)
+    if x.dim() < 1 or wq.dim() != 2 or x.shape[-1] != wq.shape[1] or wq.shape[1] == 0:
+        raise ValueError(f"shapes: x [..., K] {list(x.shape)}, wq [N, K] {list(wq.shape)}")
+    if wq.device != dev:
+        raise RuntimeError("tensors on different devices")
+    K = wq.shape[1]
+    q, s = _int8_codes(x.reshape(-1, K), -(-K // 16) * 16)
+    y = matmul_int8(q[:, :K], s, wq, ws, bias, out_dtype or x.dtype) if K % 16 == 0 else \
+        matmul_int8(q, s, _operand(wq)[0], ws, bias, out_dtype or x.dtype)
+    return y.reshape(*x.shape[:-1], wq.shape[0])
