@@ -77,7 +77,20 @@ __device__ __forceinline__ void store_from_f32(void* p, int64_t i, float v, int 
 }
 
 // silu(g) * u in fp32: the one rounding to the output's type comes after it.
-__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// With t = exp(-|g|) in [0, 1]: silu(g) = g * (g >= 0 ? 1 : t) / (1 + t), which neither
+// overflows nor divides by more than 2. t = 2^(hi + lo) with hi + lo the product
+// -|g| log2(e) carried to twice float32, so its error (3 float32 steps) does not grow with
+// |g|; about 15 instructions, a third of expf and an IEEE division.
+__device__ __forceinline__ float swiglu(float g, float u) {
+  constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.925963033500e-8f, kLn2 = 0.693147181f;
+  const float x = -fabsf(g);
+  const float hi = x * kLog2e, lo = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -hi));
+  float t, r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(t) : "f"(hi));
+  t = t == 0.0f ? 0.0f : fmaf(t, lo * kLn2, t);  // hi = -inf: lo is not a number
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + t));
+  return g * (g >= 0.0f ? r : t * r) * u;
+}
 
 }  // namespace prod
 }  // namespace gq

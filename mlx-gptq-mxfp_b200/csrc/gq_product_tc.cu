@@ -5,21 +5,27 @@
 // The weights are the M operand and the rows the N operand: D^T[channel][row]. A tile is
 // then 256 channels of one expert by 16 .. 256 of its rows (a multiple of 16, of 32 for
 // s8), so an expert's rows are cut into equal tiles and a ragged expert costs at most 15
-// (31) idle rows instead of most of a 128-row tile; and a row of D^T is one channel, so
-// SwiGLU needs no exchange: gate and up are two accumulators with the same lanes and
-// columns, combined by the thread that drains them.
+// (31) idle rows instead of most of a 128-row tile. With SwiGLU the 256 channels are 128
+// gate channels and their up channels, interleaved by the order of the tensor map's
+// dimensions: a channel's two sums sit in neighbouring lanes, and SwiGLU is one shuffle.
 //
 // A cluster of two CTAs shares a tile (cta_group::2, M = 256): each loads 128 channels of
 // the weights and half of the rows per 128-byte k-step. Persistent: pair p takes tiles p,
 // p + pairs, ... of a list that every role derives from the offsets on the device (tiles
 // per expert, scanned once into shared memory): nothing is read back to the host.
-//   warp 0       TMA: weights [expert, channel, k] and, without a row list, X (32-row boxes)
-//   warp 1       MMA issuer (even CTA), one of two TMEM accumulator sets per tile
-//   warps 2-9    drain the other set, scale / bias / SwiGLU, round once, store
-//   warps 10-13  with a row list: cp.async gathers of X rows into the swizzled stage
+//   warp 0       TMA: weights [expert, channel, k] and, without a row list, X
+//   warp 1       MMA issuer (even CTA) into one of two TMEM accumulator sets
+//   warps 4-11   drain the other set into registers; scale / bias / SwiGLU, round once, store
+//   warps 2, 3 and 12-15  with a row list: one per stage, cp.async gathers of X rows
+//
+// Precision: a tensor-core step loses up to a float32 step of the partial sum, always
+// toward zero, so one accumulator over K = 2048 drifts by 5e-6 of |y| (8 x a float32 FMA
+// chain). The 16-bit kinds therefore accumulate kChunk k-steps in TMEM and add the chunks
+// in registers, rounding to nearest (the same remedy as in gq_hessian.cu); s32 sums are
+// exact and take one chunk per tile.
 // Every wait is bounded (gq_common.cuh); a wait that gives up records GQ_ERR_TIMEOUT.
 #include <algorithm>
-#include <atomic>
+#include <type_traits>
 
 #include "gq_product.cuh"
 
@@ -27,25 +33,34 @@ namespace gq {
 namespace prod {
 namespace {
 
-constexpr int EPI_WARPS = 8, GATHER_WARPS = 4;
+constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
+constexpr int kChunk = 8;  // k-steps (64 elements each) per TMEM accumulation of the 16-bit kinds
+// Registers: the drain holds a warp's 32 x 128 sums, so the other warps give it some of
+// theirs. With the gather warps 512 threads start with 128 each: (2 * 64 + 2 * 192) * 128 =
+// 512 * 128; without, 384 with 168: (88 + 2 * 208) * 128 = 384 * 168.
+template <bool GATHER>
+constexpr int regs_few() {
+  return GATHER ? 64 : 88;
+}
+template <bool GATHER>
+constexpr int regs_drain() {
+  return GATHER ? 192 : 208;
+}
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t A_BYTES = 128 * 128;  // 128 channels x 128 bytes of k
-constexpr int BOX_ROWS = 32;             // rows of one TMA box of X
-constexpr uint32_t BOX_BYTES = BOX_ROWS * 128;
-constexpr int GATHER_LAG = 3;            // stages whose copies a gather warp has in flight
+constexpr int X_MAPS = 4;                // TMA boxes of X: 128, 64, 32 and 16 rows
 constexpr uint32_t kEvenCta = 0xFEFFFFFFu;  // shared::cluster address -> even CTA of the pair
 
-template <bool GLU>
-struct Shape {
-  static constexpr int NMAX = GLU ? 128 : 256;  // rows per tile
-  static constexpr int ACCS = GLU ? 2 : 1;      // accumulators (gate, up)
-  static constexpr uint32_t B_BYTES = uint32_t(NMAX / 2) * 128;
-  static constexpr uint32_t STAGE_BYTES = ACCS * A_BYTES + B_BYTES;
-  static constexpr int STAGES = GLU ? 5 : 6;
-  static constexpr size_t SMEM_BYTES =
-      size_t(STAGES) * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ + 8 * (kMaxExperts + 1) /*tiles, rows*/;
-};
-static_assert(Shape<false>::SMEM_BYTES <= 227 * 1024 && Shape<true>::SMEM_BYTES <= 227 * 1024, "shared memory");
+constexpr int NMAX = 256;  // rows per tile
+constexpr uint32_t B_BYTES = uint32_t(NMAX / 2) * 128;
+constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int STAGES = 6;
+constexpr int GATHER_WARPS = STAGES;
+constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ +
+                              GATHER_WARPS * (NMAX / 2) * 4 /*row lists*/ +
+                              12 * (kMaxExperts + 1) /*tiles and rows of every expert*/;
+
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -63,7 +78,9 @@ __device__ __forceinline__ void arrive_even(uint64_t* bar) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(r) : "memory");
 }
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+// mbar_wait for barriers that the other CTA of the pair arrives on.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                             int32_t* status) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -72,13 +89,10 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
-  return ok != 0;
-}
-// mbar_wait for barriers that the other CTA of the pair arrives on.
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                             int32_t* status) {
+  if (ok) return true;
   if (!mbar_wait(bar, parity, abort_flag, status)) return false;
-  return try_wait_cluster(bar, parity);  // complete already: acquires the other CTA's writes
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return true;
 }
 
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -88,11 +102,11 @@ __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x,
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(even_cta(bar))
       : "memory");
 }
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-      "%4}], [%5];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(even_cta(bar))
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+      "%4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(even_cta(bar))
       : "memory");
 }
 
@@ -134,64 +148,180 @@ __device__ __forceinline__ uint32_t instruction_desc(Kind kind, int n) {
   return types | (uint32_t(n >> 3) << 17) | (uint32_t(256 >> 4) << 24);
 }
 
+// Position in the stage ring. The waits it stands for are on the critical path of one
+// thread each: no division per step (64-bit remainders cost 15% of the whole kernel).
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void step() {
+    if (++stage == STAGES) stage = 0, phase ^= 1;
+  }
+};
+
+struct XMaps {
+  CUtensorMap box[X_MAPS];  // box[i]: 128 >> i rows
+};
+
 struct Tile {
   int64_t row0;  // first product row
   int rows;      // rows that are written
   int n;         // rows of the MMA (a multiple of the kind's step)
-  int expert, channel0;
+  int expert, block;  // block: of the 256 channels, in the order the tile holds them
 };
 
-// Tile q of the list: expert by expert, row tile by row tile, its 256-channel tiles.
-__device__ __forceinline__ Tile tile_of(int64_t q, const int32_t* first_tile, int E, int ct,
-                                        int nmax, int step, const Args& a) {
+// The experts' rows [begin, end) and the first of each one's row tiles, in shared memory.
+struct Experts {
+  int32_t *first_tile, *begin, *end;
+};
+
+// Tile q of the list: expert by expert, row tile by row tile, its channel blocks.
+__device__ __forceinline__ Tile tile_of(int q, const Experts& x, int E, int ct, int step) {
   int lo = 0, hi = E;  // last expert whose tiles begin at or before q / ct
-  const int32_t r = int32_t(q / ct);
+  const int r = q / ct;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (first_tile[mid] <= r) lo = mid; else hi = mid;
+    if (x.first_tile[mid] <= r) lo = mid; else hi = mid;
   }
-  int64_t begin, end;
-  segment(a, lo, begin, end);
-  const int64_t n = end - begin;
-  const int tiles = int((n + nmax - 1) / nmax);
-  const int per = int(((n + tiles - 1) / tiles + step - 1) / step) * step;  // <= nmax: nmax is a multiple of step
+  const int n = x.end[lo] - x.begin[lo];
+  const int tiles = (n + NMAX - 1) / NMAX;
+  const int per = ((n + tiles - 1) / tiles + step - 1) / step * step;  // <= NMAX, a multiple of step
   Tile t;
   t.expert = lo;
-  t.channel0 = int(q % ct) * 256;
-  const int64_t r0 = int64_t(r - first_tile[lo]) * per;
-  t.row0 = begin + r0;
-  t.rows = int(n - r0 < per ? (n - r0 > 0 ? n - r0 : 0) : per);
+  t.block = q - r * ct;
+  const int r0 = (r - x.first_tile[lo]) * per;
+  t.row0 = int64_t(x.begin[lo]) + r0;
+  t.rows = n - r0 < per ? (n - r0 > 0 ? n - r0 : 0) : per;
   t.n = per;
   return t;
 }
 
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (DT == GQ_BF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Two rows of one channel (packed, row j low) in this lane and of the neighbouring channel in
+// lane ^ d -> two channels of one row: row j in the lane with bit d clear, row j + 1 in the
+// other. One shuffle and one byte permutation per two elements.
+__device__ __forceinline__ uint32_t swap_rows(uint32_t w, int d, bool upper) {
+  const uint32_t got = __shfl_xor_sync(~0u, w, d);
+  return __byte_perm(w, got, upper ? 0x3276u : 0x5410u);
+}
+
+// Store v[j] = Y[row0 + j][ch], j < 32, where row0 + j < end; lanes hold consecutive
+// channels ch, those below I are real. 16-bit types: neighbouring lanes swap every other
+// row and write two channels of one row as 4 bytes (pairs: I and ldy even, Y 4-byte
+// aligned); this code runs once per tile on two warps per scheduler, so it counts
+// instructions: convert, shuffle, permute, store and a pointer step per two elements.
+template <int DT>
+__device__ __forceinline__ void store_block(const Args& a, int64_t row0, int64_t end, int64_t ch, int64_t I, bool pairs,
+                                            const float (&v)[32]) {
+  const int rows = end - row0 < 32 ? int(end - row0) : 32;
+  if (DT != GQ_F32 && pairs) {
+    const int odd = threadIdx.x & 1;  // tiles begin at even channels
+    uint8_t* p = reinterpret_cast<uint8_t*>(a.Y) + ((row0 + odd) * a.ldy + (ch - odd)) * 2;
+    const int64_t step = 4 * a.ldy;
+    const int left = ch < I ? rows - odd : 0;  // I is even: a pair's channels go together
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const uint32_t w = swap_rows(pack2<DT>(v[j], v[j + 1]), 1, odd);
+      if (j < left) *reinterpret_cast<uint32_t*>(p) = w;
+      p += step;
+    }
+  } else if (ch < I) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < rows) store_from_f32(a.Y, (row0 + j) * a.ldy + ch, v[j], DT);
+  }
+}
+
+// The same after SwiGLU: even lanes hold gate, odd lanes up sums of the channel ch that
+// lane / 2 stands for. Lanes swap every other row: the even lane finishes row j, the odd
+// lane row j + 1 of each pair; then lanes 2 apart swap rows as above.
+template <int DT>
+__device__ __forceinline__ void store_block_glu(const Args& a, int64_t row0, int64_t end, int64_t ch, int64_t I,
+                                                bool pairs, const float (&v)[32]) {
+  const int lane = threadIdx.x & 31, odd = lane & 1, odd2 = (lane >> 1) & 1;
+  const int rows = end - row0 < 32 ? int(end - row0) : 32;
+  float y[16];  // rows 2 j + odd
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float got = __shfl_xor_sync(~0u, odd ? v[2 * j] : v[2 * j + 1], 1);
+    y[j] = swiglu(odd ? got : v[2 * j], odd ? v[2 * j + 1] : got);
+  }
+  if (DT != GQ_F32 && pairs) {
+    const int first = odd + 2 * odd2;  // rows first + 4 i
+    uint8_t* p = reinterpret_cast<uint8_t*>(a.Y) + ((row0 + first) * a.ldy + (ch - odd2)) * 2;
+    const int64_t step = 8 * a.ldy;
+    const int left = ch < I ? rows - first : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w = swap_rows(pack2<DT>(y[2 * i], y[2 * i + 1]), 2, odd2);
+      if (4 * i < left) *reinterpret_cast<uint32_t*>(p) = w;
+      p += step;
+    }
+  } else if (ch < I) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (2 * j + odd < rows) store_from_f32(a.Y, (row0 + 2 * j + odd) * a.ldy + ch, y[j], DT);
+  }
+}
+
+template <bool GLU>
+__device__ __forceinline__ void store_any_block(const Args& a, int64_t row0, int64_t end, int64_t ch, int64_t I,
+                                                bool pairs, const float (&v)[32]) {
+  if constexpr (GLU) {
+    if (a.out_dtype == GQ_BF16) store_block_glu<GQ_BF16>(a, row0, end, ch, I, pairs, v);
+    else if (a.out_dtype == GQ_F16) store_block_glu<GQ_F16>(a, row0, end, ch, I, pairs, v);
+    else store_block_glu<GQ_F32>(a, row0, end, ch, I, pairs, v);
+  } else {
+    if (a.out_dtype == GQ_BF16) store_block<GQ_BF16>(a, row0, end, ch, I, pairs, v);
+    else if (a.out_dtype == GQ_F16) store_block<GQ_F16>(a, row0, end, ch, I, pairs, v);
+    else store_block<GQ_F32>(a, row0, end, ch, I, pairs, v);
+  }
+}
+
+template <bool GATHER>
+constexpr int threads() {
+  return 32 * (EPI_WARP0 + EPI_WARPS + (GATHER ? 4 : 0));
+}
+
 template <bool I8, bool GLU, bool GATHER>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EPI_WARPS + (GATHER ? 32 * GATHER_WARPS : 0), 1)
-    tc_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Args a,
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads<GATHER>(), 1)
+    tc_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ XMaps xmaps, const Args a,
               const Kind kind) {
-  typedef Shape<GLU> Sh;
-  constexpr int STAGES = Sh::STAGES, NMAX = Sh::NMAX, STEP = I8 ? 32 : 16;
+  constexpr int STEP = I8 ? 32 : 16;
   constexpr int KSTEP = I8 ? 128 : 64;  // elements per stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Sh::STAGE_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;  // [2] accumulator set complete (both CTAs)
   uint64_t* tempty = tfull + 2;      // [2] accumulator set drained by both CTAs (used in the even CTA)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int32_t* first_tile = reinterpret_cast<int32_t*>(smem + STAGES * Sh::STAGE_BYTES + 256);  // [E + 1]
+  uint32_t* gather_rows = reinterpret_cast<uint32_t*>(smem + STAGES * STAGE_BYTES + 256);  // [GATHER_WARPS][NMAX / 2]
+  Experts ex;
+  ex.first_tile = reinterpret_cast<int32_t*>(gather_rows + GATHER_WARPS * (NMAX / 2));  // [E + 1]
+  ex.begin = ex.first_tile + kMaxExperts + 1;
+  ex.end = ex.begin + kMaxExperts + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
   const int E = int(a.E), pairs = int(gridDim.x >> 1), pair = int(blockIdx.x >> 1);
   const int64_t I = GLU ? a.N / 2 : a.N;
-  const int ct = int((I + 255) / 256);
+  const int ct = int((I + (GLU ? 127 : 255)) / (GLU ? 128 : 256));  // channel blocks
   const int KT = int((a.K + KSTEP - 1) / KSTEP);
+  const int chunk = I8 ? KT : kChunk;  // k-steps per accumulation
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1 + (GATHER ? 2 * GATHER_WARPS : 0));
+      mbar_init(&full[s], 1 + (GATHER ? 2 : 0));  // expect_tx; a gather warp of each CTA
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -206,194 +336,242 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EPI_WARPS 
                  "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
-  if (warp == 2) {  // exclusive scan of the experts' row tiles
-    int32_t carry = 0;
+  if (warp == 2) {
+    // Rows of every expert and the exclusive scan of their tiles. Offsets that run backwards
+    // are raised to the largest before them, so that the tiles stay within S rows whatever
+    // the offsets hold.
+    int32_t carry = 0, reached = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const int e = e0 + lane;
       int64_t begin = 0, end = 0;
       if (e < E) segment(a, e, begin, end);
-      const int32_t mine = int32_t((end - begin + NMAX - 1) / NMAX);
+      int32_t stop = int32_t(end);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int32_t o = __shfl_up_sync(~0u, stop, d);
+        if (lane >= d) stop = max(stop, o);
+      }
+      stop = max(stop, reached);
+      int32_t start = __shfl_up_sync(~0u, stop, 1);
+      start = max(int32_t(begin), lane ? start : reached);
+      if (start > stop) start = stop;
+      const int32_t mine = (stop - start + NMAX - 1) / NMAX;
       int32_t incl = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int32_t o = __shfl_up_sync(~0u, incl, d);
         if (lane >= d) incl += o;
       }
-      if (e < E) first_tile[e] = carry + incl - mine;
+      if (e < E) ex.first_tile[e] = carry + incl - mine, ex.begin[e] = start, ex.end[e] = stop;
       carry += __shfl_sync(~0u, incl, 31);
+      reached = __shfl_sync(~0u, stop, 31);
     }
-    if (lane == 0) first_tile[E] = carry;
+    if (lane == 0) ex.first_tile[E] = carry;
   }
   tc_fence_before();
   __syncthreads();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int64_t tiles = int64_t(first_tile[E]) * ct;
+  const int tiles = ex.first_tile[E] * ct;  // below 2^31: checked by the host for any offsets
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp >= EPI_WARP0 && warp < EPI_WARP0 + EPI_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(regs_drain<GATHER>()));
+    // TMEM lane quarter warp % 4 (channels); every other 32 of the tile's columns (rows)
+    typedef typename std::conditional<I8, int32_t, float>::type Sum;
+    const int qw = warp & 3, part = (warp - EPI_WARP0) >> 2;
+    const uint32_t lane_base = uint32_t(qw * 32) << 16;
+    const bool in_pairs = a.out_dtype != GQ_F32 && I % 2 == 0 && a.ldy % 2 == 0 &&
+                          (reinterpret_cast<uintptr_t>(a.Y) & 3u) == 0;
+    int n_chunk = 0;
+    bool ok = true;
+    for (int q = pair; q < tiles && ok; q += pairs) {
+      const Tile t = tile_of(q, ex, E, ct, STEP);
+      Sum acc[4][32];
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[b][j] = Sum(0);
+      for (int k0 = 0; k0 < KT; k0 += chunk, ++n_chunk) {
+        const int buf = n_chunk & 1;
+        if (!mbar_wait(&tfull[buf], (n_chunk >> 1) & 1, abort_flag, a.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int c = part * 32 + 64 * b;
+          if (c < t.rows) {
+            uint32_t r[32];
+            tmem_ld32(tmem + lane_base + uint32_t(buf * 256 + c), r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if constexpr (I8)
+                acc[b][j] = int32_t(r[j]);  // one chunk
+              else
+                acc[b][j] = acc[b][j] + __uint_as_float(r[j]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_even(&tempty[buf]);
+      }
+      if (!ok) break;
+      const int row128 = int(rank) * 128 + qw * 32 + lane;  // of the tile's 256 channels
+      const int64_t ch = GLU ? t.block * 128 + row128 / 2 : t.block * 256 + row128;
+      float ws = 1.0f, bias = 0.0f;
+      if (I8 && ch < I) {
+        ws = a.ws[t.expert * a.N + ch + (GLU && lane & 1 ? I : 0)];
+        if (a.bias) bias = load_as_f32(a.bias, ch, a.bias_dtype);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int c = part * 32 + 64 * b;
+        if (c < t.rows) {
+          float xs_lane = 0.0f;
+          if (I8 && c + lane < t.rows) {
+            const int64_t src = source_row(a, t.row0 + c + lane);
+            xs_lane = src >= 0 ? a.xs[src] : 0.0f;
+          }
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if constexpr (I8)
+              v[j] = float(acc[b][j]) * __shfl_sync(~0u, xs_lane, j) * ws + bias;
+            else
+              v[j] = acc[b][j];
+          }
+          store_any_block<GLU>(a, t.row0 + c, t.row0 + t.rows, ch, I, in_pairs, v);
+        }
+      }
+    }
+    if (a.zero_behind) {
+      const int64_t first = rows_end(a), count = (a.S - first) * I;
+      for (int64_t i = int64_t(blockIdx.x) * (32 * EPI_WARPS) + threadIdx.x - 32 * EPI_WARP0; i < count;
+           i += int64_t(gridDim.x) * (32 * EPI_WARPS))
+        store_from_f32(a.Y, (first + i / I) * a.ldy + i % I, 0.0f, a.out_dtype);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(regs_few<GATHER>()));
+    if (warp == 0 && lane == 0) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
-      if (!GATHER) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&xmap)) : "memory");
-      int64_t it = 0;
-      bool ok = true;
-      for (int64_t q = pair; q < tiles && ok; q += pairs) {
-        const Tile t = tile_of(q, first_tile, E, ct, NMAX, STEP, a);
-        const int half = t.n / 2, boxes = GATHER ? 0 : (half + BOX_ROWS - 1) / BOX_ROWS;
-        const uint32_t bytes = Sh::ACCS * A_BYTES + uint32_t(boxes) * BOX_BYTES;
-        const int ch = t.channel0 + int(rank) * 128, y = int(t.row0) + int(rank) * half;
-        for (int kt = 0; kt < KT; ++kt, ++it) {
-          const int s = int(it % STAGES);
-          if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, a.status)) {
+      if (!GATHER)
+        for (int b = 0; b < X_MAPS; ++b)
+          asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&xmaps.box[b])) : "memory");
+      Ring ring;
+      bool ok = true, lapped = false;
+      for (int q = pair; q < tiles && ok; q += pairs) {
+        const Tile t = tile_of(q, ex, E, ct, STEP);
+        const int half = t.n / 2, x_rows = GATHER ? 0 : (half + 15) / 16 * 16;  // <= 128
+        const uint32_t bytes = A_BYTES + uint32_t(x_rows) * 128;
+        const int ch = (t.block * 2 + int(rank)) * (GLU ? 64 : 128), y = int(t.row0) + int(rank) * half;
+        for (int kt = 0; kt < KT; ++kt) {
+          const int s = ring.stage;
+          if (!mbar_wait(&empty[s], ring.phase ^ 1, abort_flag, a.status)) {
             ok = false;
             break;
           }
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * bytes);  // both CTAs' bytes
-          uint8_t* st = smem + s * Sh::STAGE_BYTES;
-          tma_3d(st, &wmap, kt * KSTEP, ch, t.expert, &full[s]);
-          if (GLU) tma_3d(st + A_BYTES, &wmap, kt * KSTEP, int(I) + ch, t.expert, &full[s]);
-          for (int b = 0; b < boxes; ++b)
-            tma_2d(st + Sh::ACCS * A_BYTES + b * BOX_BYTES, &xmap, kt * KSTEP, y + b * BOX_ROWS, &full[s]);
+          uint8_t* st = smem + s * STAGE_BYTES;
+          tma_4d(st, &wmap, kt * KSTEP, 0, ch, t.expert, &full[s]);  // (k, gate / up, channel, expert)
+          // few large boxes: each costs the TMA unit and this thread a fixed time
+          for (int b = 0, r = 0; b < X_MAPS; ++b)
+            if (x_rows & (128 >> b)) {
+              tma_2d(st + A_BYTES + r * 128, &xmaps.box[b], kt * KSTEP, y + r, &full[s]);
+              r += 128 >> b;
+            }
+          ring.step();
+          lapped |= ring.stage == 0;
         }
       }
       if (*abort_flag && rank == 0) {  // let copies already in flight land before the CTA exits
         volatile int never = 0;
-        for (int64_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-          mbar_wait(&full[i % STAGES], (i / STAGES) & 1, &never, nullptr);
+        for (int i = 0; i < STAGES; ++i)  // the last load of stage i: this lap's, or the lap's before
+          if (i < ring.stage || lapped)
+            mbar_wait(&full[i], i < ring.stage ? ring.phase : ring.phase ^ 1, &never, nullptr);
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      int64_t it = 0;
-      int n_tile = 0;
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      Ring ring;
+      int n_chunk = 0;
       bool ok = true;
-      for (int64_t q = pair; q < tiles && ok; q += pairs, ++n_tile) {
-        const Tile t = tile_of(q, first_tile, E, ct, NMAX, STEP, a);
+      const uint64_t desc = umma_desc_sw128(smem_u32(smem), 16, 1024);  // + (byte offset >> 4)
+      for (int q = pair; q < tiles && ok; q += pairs) {
+        const Tile t = tile_of(q, ex, E, ct, STEP);
         const uint32_t idesc = instruction_desc(kind, t.n);
-        const int buf = n_tile & 1;
-        if (!wait_cluster(&tempty[buf], ((n_tile >> 1) & 1) ^ 1, abort_flag, a.status)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + uint32_t(buf * 256);
-        for (int kt = 0; kt < KT; ++kt, ++it) {
-          const int s = int(it % STAGES);
-          if (!wait_cluster(&full[s], (it / STAGES) & 1, abort_flag, a.status)) {
+        for (int k0 = 0; k0 < KT && ok; k0 += chunk, ++n_chunk) {
+          const int buf = n_chunk & 1, k1 = k0 + chunk < KT ? k0 + chunk : KT;
+          if (!wait_cluster(&tempty[buf], ((n_chunk >> 1) & 1) ^ 1, abort_flag, a.status)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + s * Sh::STAGE_BYTES), b0 = a0 + Sh::ACCS * A_BYTES;
+          const uint32_t d = tmem + uint32_t(buf * 256);
+          for (int kt = k0; kt < k1; ++kt) {
+            const int s = ring.stage;
+            if (!wait_cluster(&full[s], ring.phase, abort_flag, a.status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t ad = desc + uint32_t(s) * (STAGE_BYTES >> 4), bd = ad + (A_BYTES >> 4);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {  // 32 bytes of k each, inside the 128-byte swizzle atom
-            const uint64_t bd = umma_desc_sw128(b0 + kk * 32, 16, 1024);
-            mma<I8>(d, umma_desc_sw128(a0 + kk * 32, 16, 1024), bd, idesc, kt != 0 || kk != 0);
-            if (GLU) mma<I8>(d + 128, umma_desc_sw128(a0 + A_BYTES + kk * 32, 16, 1024), bd, idesc, kt != 0 || kk != 0);
+            for (int kk = 0; kk < 4; ++kk) {  // 32 bytes of k each, inside the 128-byte swizzle atom
+              const uint32_t more = kt != k0 || kk != 0;
+              mma<I8>(d, ad + 2 * kk, bd + 2 * kk, idesc, more);
+            }
+            commit(&empty[s]);  // frees the stage once these MMAs have read it
+            ring.step();
           }
-          commit(&empty[s]);  // frees the stage once these MMAs have read it
+          if (ok) commit(&tfull[buf]);
         }
-        if (ok) commit(&tfull[buf]);
       }
-    }
-  } else if (warp < 2 + EPI_WARPS) {
-    // TMEM lane quarter warp % 4 (channels), half of the tile's columns (rows)
-    const int qw = warp & 3, part = (warp - 2) >> 2;
-    const uint32_t lane_base = uint32_t(qw * 32) << 16;
-    int n_tile = 0;
-    for (int64_t q = pair; q < tiles; q += pairs, ++n_tile) {
-      const Tile t = tile_of(q, first_tile, E, ct, NMAX, STEP, a);
-      const int buf = n_tile & 1;
-      if (!mbar_wait(&tfull[buf], (n_tile >> 1) & 1, abort_flag, a.status)) break;
-      tc_fence_after();
-      const int64_t ch = t.channel0 + int(rank) * 128 + qw * 32 + lane;
-      const bool live = ch < I;
-      float ws = 1.0f, ws_up = 1.0f, bias = 0.0f;
-      if (live && I8) {
-        ws = a.ws[t.expert * a.N + ch];
-        if (GLU) ws_up = a.ws[t.expert * a.N + I + ch];
-      }
-      if (live && a.bias) bias = load_as_f32(a.bias, ch, a.bias_dtype);
-      for (int c = part * 32; c < t.rows; c += 64) {
-        uint32_t r[32], u[GLU ? 32 : 1];
-        tmem_ld32(tmem + lane_base + uint32_t(buf * 256 + c), r);
-        if constexpr (GLU) tmem_ld32(tmem + lane_base + uint32_t(buf * 256 + 128 + c), u);
-        float xs_lane = 0.0f;
-        if (I8 && c + lane < t.rows) {
-          const int64_t src = source_row(a, t.row0 + c + lane);
-          xs_lane = src >= 0 ? a.xs[src] : 0.0f;
+    } else if (GATHER && warp != 0 && warp != 1) {
+      // Gather warp w copies the rows of stage w, whole, and hands it over when they have
+      // landed: about 2 us from a free stage to a full one, in which the tensor core works
+      // on the other five (four warps: a third slower).
+      constexpr uint32_t kNone = 0xFFFFFFFFu;
+      const int w = warp < EPI_WARP0 ? warp - 2 : warp - (EPI_WARP0 + EPI_WARPS) + 2, chunk16 = lane & 7, r_lane = lane >> 3;
+      uint32_t* source = gather_rows + w * (NMAX / 2);  // this CTA's rows of the tile: X offset / 16, kNone: zeros
+      const int64_t kbytes = a.K * (I8 ? 1 : 2);
+      const uint32_t ld16 = uint32_t(a.ldx >> 4);
+      const uint32_t swz0 = uint32_t(chunk16 ^ r_lane) << 4, swz1 = uint32_t(chunk16 ^ (r_lane + 4)) << 4;
+      Ring ring;
+      bool ok = true;
+      for (int q = pair; q < tiles && ok; q += pairs) {
+        const Tile t = tile_of(q, ex, E, ct, STEP);
+        const int half = t.n / 2;  // a multiple of 8
+        __syncwarp();
+        for (int r = lane; r < half; r += 32) {
+          const int p = int(rank) * half + r;
+          const int64_t x = p < t.rows ? source_row(a, t.row0 + p) : -1;
+          source[r] = x >= 0 ? uint32_t(x) * ld16 : kNone;
         }
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          float v, up = 0.0f;
-          if (I8) {
-            const float xs = __shfl_sync(~0u, xs_lane, j);
-            v = float(int32_t(r[j])) * xs * ws;
-            if constexpr (GLU) up = float(int32_t(u[j])) * xs * ws_up;
-          } else {
-            v = __uint_as_float(r[j]);
-            if constexpr (GLU) up = __uint_as_float(u[j]);
+        __syncwarp();
+        for (int kt = 0; kt < KT; ++kt, ring.step()) {
+          const int s = ring.stage;
+          if (s != w) continue;
+          if (!mbar_wait(&empty[s], ring.phase ^ 1, abort_flag, a.status)) {
+            ok = false;
+            break;
           }
-          v = v + bias;
-          if (GLU) v = swiglu(v, up);
-          if (live && c + j < t.rows) store_from_f32(a.Y, (t.row0 + c + j) * a.ldy + ch, v, a.out_dtype);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_even(&tempty[buf]);
-    }
-    if (a.zero_behind) {
-      const int64_t first = rows_end(a), count = (a.S - first) * I;
-      for (int64_t i = int64_t(blockIdx.x) * (32 * EPI_WARPS) + threadIdx.x - 64; i < count;
-           i += int64_t(gridDim.x) * (32 * EPI_WARPS))
-        store_from_f32(a.Y, (first + i / I) * a.ldy + i % I, 0.0f, a.out_dtype);
-    }
-  } else if (GATHER) {
-    const int tid = threadIdx.x - (64 + 32 * EPI_WARPS), chunk = tid & 7, r_base = tid >> 3;
-    constexpr int RPT = NMAX / 2 / 16;  // rows per thread
-    const int64_t kbytes = a.K * (I8 ? 1 : 2);
-    int64_t it = 0, arrived = 0;
-    bool ok = true;
-    for (int64_t q = pair; q < tiles && ok; q += pairs) {
-      const Tile t = tile_of(q, first_tile, E, ct, NMAX, STEP, a);
-      const int half = t.n / 2;
-      const uint8_t* src[RPT];
-#pragma unroll
-      for (int i = 0; i < RPT; ++i) {
-        const int r = int(rank) * half + r_base + 16 * i;  // row of the tile
-        const int64_t x = r_base + 16 * i < half && r < t.rows ? source_row(a, t.row0 + r) : -1;
-        src[i] = x >= 0 ? a.X + x * a.ldx + chunk * 16 : nullptr;
-      }
-      for (int kt = 0; kt < KT; ++kt, ++it) {
-        const int s = int(it % STAGES);
-        if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, a.status)) {
-          ok = false;
-          break;
-        }
-        const uint32_t dst = smem_u32(smem + s * Sh::STAGE_BYTES + Sh::ACCS * A_BYTES);
-        const bool in = kt * 128 + chunk * 16 < kbytes;
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-          const int r = r_base + 16 * i;
-          if (r < half) {
-            const bool on = in && src[i] != nullptr;
-            cp_async16(dst + r * 128 + ((chunk ^ (r & 7)) << 4), on ? src[i] + kt * 128 : a.X, on);
+          const uint32_t dst = smem_u32(smem + s * STAGE_BYTES + A_BYTES) + r_lane * 128;
+          const bool in = kt * 128 + chunk16 * 16 < kbytes;
+          const uint8_t* x = a.X + kt * 128 + chunk16 * 16;
+#pragma unroll 4
+          for (int r = 0; r < half; r += 8) {  // 8 lanes per row: 128 contiguous bytes
+            const uint32_t s0 = source[r + r_lane], s1 = source[r + r_lane + 4];
+            const bool on0 = in && s0 != kNone, on1 = in && s1 != kNone;
+            cp_async16(dst + r * 128 + swz0, on0 ? x + uint64_t(s0) * 16 : a.X, on0);
+            cp_async16(dst + r * 128 + 512 + swz1, on1 ? x + uint64_t(s1) * 16 : a.X, on1);
           }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (it >= GATHER_LAG) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(GATHER_LAG) : "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads what was copied
           __syncwarp();
-          if (lane == 0) arrive_even(&full[arrived % STAGES]);
-          ++arrived;
+          if (lane == 0) arrive_even(&full[s]);
         }
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    for (; arrived < it; ++arrived)
-      if (lane == 0) arrive_even(&full[arrived % STAGES]);
   }
   tc_fence_before();
   __syncthreads();
@@ -411,7 +589,7 @@ int encode(CUtensorMap* map, const void* base, Kind kind, int rank, const cuuint
     set_last_error("cuTensorMapEncodeTiled unavailable");
     return GQ_ERR_CUDA;
   }
-  const cuuint32_t estr[3] = {1, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUtensorMapDataType type = kind == S8     ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                    : kind == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -426,19 +604,18 @@ int encode(CUtensorMap* map, const void* base, Kind kind, int rank, const cuuint
 }
 
 template <bool I8, bool GLU, bool GATHER>
-int launch(const CUtensorMap& wmap, const CUtensorMap& xmap, const Args& a, Kind kind, unsigned grid, cudaStream_t s) {
+int launch(const CUtensorMap& wmap, const XMaps& xmaps, const Args& a, Kind kind, unsigned grid, cudaStream_t s) {
   auto* k = tc_kernel<I8, GLU, GATHER>;
-  GQ_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<GLU>::SMEM_BYTES)));
-  const int threads = 64 + 32 * EPI_WARPS + (GATHER ? 32 * GATHER_WARPS : 0);
-  k<<<grid, threads, Shape<GLU>::SMEM_BYTES, s>>>(wmap, xmap, a, kind);
+  GQ_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_BYTES)));
+  k<<<grid, threads<GATHER>(), SMEM_BYTES, s>>>(wmap, xmaps, a, kind);
   return check_launch("tc_kernel");
 }
 
 template <bool I8, bool GLU>
-int launch_gather(const CUtensorMap& wmap, const CUtensorMap& xmap, const Args& a, Kind kind, unsigned grid,
+int launch_gather(const CUtensorMap& wmap, const XMaps& xmaps, const Args& a, Kind kind, unsigned grid,
                   cudaStream_t s) {
-  return a.rows ? launch<I8, GLU, true>(wmap, xmap, a, kind, grid, s)
-                : launch<I8, GLU, false>(wmap, xmap, a, kind, grid, s);
+  return a.rows ? launch<I8, GLU, true>(wmap, xmaps, a, kind, grid, s)
+                : launch<I8, GLU, false>(wmap, xmaps, a, kind, grid, s);
 }
 
 }  // namespace
@@ -446,31 +623,38 @@ int launch_gather(const CUtensorMap& wmap, const CUtensorMap& xmap, const Args& 
 int launch_tc(const Args& a, Kind kind, bool glu, cudaStream_t s) {
   const cuuint64_t es = kind == S8 ? 1 : 2;
   const cuuint32_t kbox = cuuint32_t(128 / es);
-  CUtensorMap wmap, xmap;
-  const cuuint64_t wdims[3] = {cuuint64_t(a.K), cuuint64_t(a.N), cuuint64_t(a.E)};
-  const cuuint64_t wstrides[2] = {cuuint64_t(a.ldw), cuuint64_t(a.stride_w)};
-  const cuuint32_t wbox[3] = {kbox, 128, 1};
-  int st = encode(&wmap, a.W, kind, 3, wdims, wstrides, wbox);
+  CUtensorMap wmap;
+  XMaps xmaps;
+  // (k, gate / up, channel, expert): gate and up channels interleaved; plain: a dimension of 1
+  const cuuint64_t I = cuuint64_t(glu ? a.N / 2 : a.N), halves = glu ? 2 : 1;
+  const cuuint64_t wdims[4] = {cuuint64_t(a.K), halves, I, cuuint64_t(a.E)};
+  const cuuint64_t wstrides[3] = {glu ? I * cuuint64_t(a.ldw) : cuuint64_t(a.ldw), cuuint64_t(a.ldw),
+                                  cuuint64_t(a.stride_w)};
+  const cuuint32_t wbox[4] = {kbox, cuuint32_t(halves), cuuint32_t(128 / halves), 1};
+  int st = encode(&wmap, a.W, kind, 4, wdims, wstrides, wbox);
   if (st != GQ_OK) return st;
-  xmap = wmap;
-  if (!a.rows) {
+  for (int b = 0; b < X_MAPS; ++b) {
+    xmaps.box[b] = wmap;  // not read with a row list
+    if (a.rows) continue;
     const cuuint64_t xdims[2] = {cuuint64_t(a.K), cuuint64_t(a.n_src)};
     const cuuint64_t xstrides[1] = {cuuint64_t(a.ldx)};
-    const cuuint32_t xbox[2] = {kbox, cuuint32_t(BOX_ROWS)};
-    st = encode(&xmap, a.X, kind, 2, xdims, xstrides, xbox);
+    const cuuint32_t xbox[2] = {kbox, cuuint32_t(128 >> b)};
+    st = encode(&xmaps.box[b], a.X, kind, 2, xdims, xstrides, xbox);
     if (st != GQ_OK) return st;
   }
   int dev = 0, sms = 0;
   GQ_CUDA_TRY(cudaGetDevice(&dev));
   GQ_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const int64_t I = glu ? a.N / 2 : a.N, nmax = glu ? 128 : 256;
-  const int64_t most = ((I + 255) / 256) * (a.S / nmax + std::min(a.S, a.E));  // at least the number of tiles
+  const int64_t blocks = (a.N + 255) / 256;
+  const int64_t most = blocks * (a.S / NMAX + std::min(a.S, a.E));  // at least the number of tiles
+  GQ_REQUIRE(most < (int64_t(1) << 31) - 65536, "product: too many tiles");
+  GQ_REQUIRE(!a.rows || a.n_src * (a.ldx >> 4) < 0xFFFFFFFFll, "product: X of a row list is limited to 64 GB");
   const unsigned grid = unsigned(2 * std::min<int64_t>(std::max(sms / 2, 1), std::max<int64_t>(most, 1)));
   if (kind == S8)
-    return glu ? launch_gather<true, true>(wmap, xmap, a, kind, grid, s)
-               : launch_gather<true, false>(wmap, xmap, a, kind, grid, s);
-  return glu ? launch_gather<false, true>(wmap, xmap, a, kind, grid, s)
-             : launch_gather<false, false>(wmap, xmap, a, kind, grid, s);
+    return glu ? launch_gather<true, true>(wmap, xmaps, a, kind, grid, s)
+               : launch_gather<true, false>(wmap, xmaps, a, kind, grid, s);
+  return glu ? launch_gather<false, true>(wmap, xmaps, a, kind, grid, s)
+             : launch_gather<false, false>(wmap, xmaps, a, kind, grid, s);
 }
 
 }  // namespace prod
