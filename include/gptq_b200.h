@@ -321,10 +321,13 @@ int gq_combine_slots(const void* y, int dtype, int64_t S, int64_t ldy, const int
  * offsets[E] on are written as zeros with zero_behind != 0, else left as they were.
  * K, ldx, ldw, stride_w multiples of 8, X and W 16-byte aligned; E <= 1024.
  * engine: -1 chosen by sizes, 0 the few-rows kernel, 1 the tcgen05 kernel.
+ * workspace: needed with rows, where the tcgen05 kernel runs (the rows are gathered into
+ * it first): gq_matmul_workspace_size bytes, 16-byte aligned; 0: none.
  * status: optional device int32 (as in gq_prepare_hinv). */
+size_t gq_matmul_workspace_size(int64_t S, int64_t E, int64_t K, int element_bytes, int engine);
 int gq_matmul_grouped(const void* X, int64_t n, int64_t ldx, const int32_t* rows, int64_t S, const int64_t* offsets,
                       int64_t E, const void* W, int64_t N, int64_t K, int64_t ldw, int64_t stride_w, int dtype,
-                      int glu, void* Y, int64_t ldy, int zero_behind, int engine, int32_t* status, void* stream);
+                      int glu, void* Y, int64_t ldy, int zero_behind, int engine, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* The same for 8-bit codes: z = (Xq Wq^T, exact 32-bit sums) * xs[row] * ws[e, channel]
  * (+ bias[channel], dense only: offsets NULL, no glu) in fp32, rounded once to out_dtype
@@ -333,7 +336,8 @@ int gq_matmul_grouped(const void* X, int64_t n, int64_t ldx, const int32_t* rows
 int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, const int32_t* rows, int64_t S,
                    const int64_t* offsets, int64_t E, const int8_t* Wq, const float* ws, int64_t N, int64_t K,
                    int64_t ldw, int64_t stride_w, const void* bias, int bias_dtype, int glu, void* Y, int out_dtype,
-                   int64_t ldy, int zero_behind, int engine, int32_t* status, void* stream);
+                   int64_t ldy, int zero_behind, int engine, void* workspace, size_t workspace_bytes, int32_t* status,
+                   void* stream);
 
 /* ------------------------------------------------------------------------
  * Packing (mlx_gptq/packing.py, mlx_gptq/artifacts.py)

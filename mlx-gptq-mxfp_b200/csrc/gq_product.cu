@@ -9,9 +9,10 @@ namespace {
 
 // The few-rows kernel reads the weights of an expert once per 8 .. 32 rows, the tcgen05
 // kernel once per 128 .. 256: the first while a busy expert's rows fit one pass.
-bool few_rows(const Args& a) { return a.S <= 8 * (a.offsets ? a.E : 1); }
+bool by_rows(int64_t S, int64_t E, int engine) { return engine == 0 || (engine < 0 && S <= 8 * E); }
 
-int run(const char* what, const Args& a, Kind kind, bool glu, int engine, cudaStream_t s) {
+int run(const char* what, const Args& a, Kind kind, bool glu, int engine, void* workspace, size_t workspace_bytes,
+        cudaStream_t s) {
   const int64_t es = kind == S8 ? 1 : 2;
   const int64_t I = glu ? a.N / 2 : a.N;
   GQ_REQUIRE(a.S >= 0 && a.S < (int64_t(1) << 31) && a.n_src >= 0 && a.n_src < (int64_t(1) << 31),
@@ -32,7 +33,11 @@ int run(const char* what, const Args& a, Kind kind, bool glu, int engine, cudaSt
   if (a.S == 0) return GQ_OK;
   GQ_REQUIRE(a.X && a.W && a.Y && a.n_src > 0, "%s: null pointer", what);
   GQ_REQUIRE(aligned16(a.X) && aligned16(a.W), "%s: X and W must be 16-byte aligned", what);
-  return (engine == 0 || (engine < 0 && few_rows(a))) ? launch_rows(a, kind, glu, s) : launch_tc(a, kind, glu, s);
+  if (by_rows(a.S, a.E, engine)) return launch_rows(a, kind, glu, s);
+  const size_t need = a.rows ? size_t(a.S) * size_t(a.K * es) : 0;
+  GQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
+             "%s: workspace too small (%zu < %zu)", what, workspace_bytes, need);
+  return launch_tc(a, kind, glu, workspace, s);
 }
 
 }  // namespace
@@ -42,24 +47,30 @@ int run(const char* what, const Args& a, Kind kind, bool glu, int engine, cudaSt
 using namespace gq;
 using namespace gq::prod;
 
+extern "C" size_t gq_matmul_workspace_size(int64_t S, int64_t E, int64_t K, int element_bytes, int engine) {
+  if (S <= 0 || E <= 0 || K <= 0) return 0;
+  return by_rows(S, E, engine) ? 0 : size_t(S) * size_t(K) * size_t(element_bytes);
+}
+
 extern "C" int gq_matmul_grouped(const void* X, int64_t n, int64_t ldx, const int32_t* rows, int64_t S,
                                  const int64_t* offsets, int64_t E, const void* W, int64_t N, int64_t K, int64_t ldw,
                                  int64_t stride_w, int dtype, int glu, void* Y, int64_t ldy, int zero_behind,
-                                 int engine, int32_t* status, void* stream) {
+                                 int engine, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   GQ_REQUIRE(dtype == GQ_BF16 || dtype == GQ_F16, "gq_matmul_grouped: rows and weights are bf16 or f16 (dtype %d)",
              dtype);
   Args a = {};
   a.X = (const uint8_t*)X, a.n_src = n, a.ldx = 2 * ldx, a.rows = rows, a.offsets = offsets, a.E = E, a.S = S;
   a.W = (const uint8_t*)W, a.N = N, a.K = K, a.ldw = 2 * ldw, a.stride_w = 2 * stride_w;
   a.Y = Y, a.ldy = ldy, a.out_dtype = dtype, a.zero_behind = zero_behind, a.status = status;
-  return run("gq_matmul_grouped", a, dtype == GQ_BF16 ? BF16 : F16, glu != 0, engine, (cudaStream_t)stream);
+  return run("gq_matmul_grouped", a, dtype == GQ_BF16 ? BF16 : F16, glu != 0, engine, workspace,
+             workspace_bytes, (cudaStream_t)stream);
 }
 
 extern "C" int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, const int32_t* rows,
                               int64_t S, const int64_t* offsets, int64_t E, const int8_t* Wq, const float* ws,
                               int64_t N, int64_t K, int64_t ldw, int64_t stride_w, const void* bias, int bias_dtype,
                               int glu, void* Y, int out_dtype, int64_t ldy, int zero_behind, int engine,
-                              int32_t* status, void* stream) {
+                              void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   GQ_REQUIRE(out_dtype == GQ_BF16 || out_dtype == GQ_F16 || out_dtype == GQ_F32, "gq_matmul_int8: out dtype %d",
              out_dtype);
   GQ_REQUIRE(!bias || bias_dtype == GQ_BF16 || bias_dtype == GQ_F16 || bias_dtype == GQ_F32,
@@ -73,5 +84,6 @@ extern "C" int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int6
   a.W = (const uint8_t*)Wq, a.N = N, a.K = K, a.ldw = ldw, a.stride_w = stride_w;
   a.xs = xs, a.ws = ws, a.bias = bias, a.bias_dtype = bias_dtype;
   a.Y = Y, a.ldy = ldy, a.out_dtype = out_dtype, a.zero_behind = zero_behind, a.status = status;
-  return run("gq_matmul_int8", a, S8, glu != 0, engine, (cudaStream_t)stream);
+  return run("gq_matmul_int8", a, S8, glu != 0, engine, workspace,
+             workspace_bytes, (cudaStream_t)stream);
 }

@@ -35,7 +35,8 @@ struct Args {
 };
 
 int launch_rows(const Args& a, Kind kind, bool glu, cudaStream_t s);
-int launch_tc(const Args& a, Kind kind, bool glu, cudaStream_t s);
+// gathered: with a row list, S * K elements, 16-byte aligned.
+int launch_tc(const Args& a, Kind kind, bool glu, void* gathered, cudaStream_t s);
 
 // Rows of expert e, whatever the offsets hold: 0 <= begin <= end <= S.
 __device__ __forceinline__ void segment(const Args& a, int64_t e, int64_t& begin, int64_t& end) {

@@ -13,10 +13,15 @@
 // the weights and half of the rows per 128-byte k-step. Persistent: pair p takes tiles p,
 // p + pairs, ... of a list that every role derives from the offsets on the device (tiles
 // per expert, scanned once into shared memory): nothing is read back to the host.
-//   warp 0       TMA: weights [expert, channel, k] and, without a row list, X
+//   warp 0       TMA: weights [expert, channel, k] and X
 //   warp 1       MMA issuer (even CTA) into one of two TMEM accumulator sets
 //   warps 4-11   drain the other set into registers; scale / bias / SwiGLU, round once, store
-//   warps 2, 3 and 12-15  with a row list: one per stage, cp.async gathers of X rows
+// A row list is applied by a copy before the launch (gather_kernel). Gathering inside the
+// kernel, six warps with cp.async beside the TMA producer, was built and measured: 541 us
+// against 457 + 55 us for 65536 rows of K = 2048 times 128 experts of 1536 channels.
+//
+// What bounds it: with 256 x 256 tiles every SM takes 32 KB per 512 cycles of MMA; the
+// loads alone sustain 47 bytes per cycle and SM (13 TB/s from L2 over the GPU), 690 cycles.
 //
 // Precision: a tensor-core step loses up to a float32 step of the partial sum, always
 // toward zero, so one accumulator over K = 2048 drifts by 5e-6 of |y| (8 x a float32 FMA
@@ -36,16 +41,8 @@ namespace {
 constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
 constexpr int kChunk = 8;  // k-steps (64 elements each) per TMEM accumulation of the 16-bit kinds
 // Registers: the drain holds a warp's 32 x 128 sums, so the other warps give it some of
-// theirs. With the gather warps 512 threads start with 128 each: (2 * 64 + 2 * 192) * 128 =
-// 512 * 128; without, 384 with 168: (88 + 2 * 208) * 128 = 384 * 168.
-template <bool GATHER>
-constexpr int regs_few() {
-  return GATHER ? 64 : 88;
-}
-template <bool GATHER>
-constexpr int regs_drain() {
-  return GATHER ? 192 : 208;
-}
+// theirs: (88 + 2 * 208) * 128 = 384 threads * 168.
+constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS), REGS_FEW = 88, REGS_DRAIN = 208;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t A_BYTES = 128 * 128;  // 128 channels x 128 bytes of k
 constexpr int X_MAPS = 4;                // TMA boxes of X: 128, 64, 32 and 16 rows
@@ -55,9 +52,7 @@ constexpr int NMAX = 256;  // rows per tile
 constexpr uint32_t B_BYTES = uint32_t(NMAX / 2) * 128;
 constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int STAGES = 6;
-constexpr int GATHER_WARPS = STAGES;
 constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ +
-                              GATHER_WARPS * (NMAX / 2) * 4 /*row lists*/ +
                               12 * (kMaxExperts + 1) /*tiles and rows of every expert*/;
 
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
@@ -134,11 +129,6 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
           smem_u32(bar)),
       "h"(uint16_t(3))
       : "memory");
-}
-
-// 16 bytes global -> shared, zeros where on is false (nothing is read then).
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 
 // Instruction descriptor: M = 256, N rows, both operands K-major.
@@ -286,13 +276,8 @@ __device__ __forceinline__ void store_any_block(const Args& a, int64_t row0, int
   }
 }
 
-template <bool GATHER>
-constexpr int threads() {
-  return 32 * (EPI_WARP0 + EPI_WARPS + (GATHER ? 4 : 0));
-}
-
-template <bool I8, bool GLU, bool GATHER>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads<GATHER>(), 1)
+template <bool I8, bool GLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ XMaps xmaps, const Args a,
               const Kind kind) {
   constexpr int STEP = I8 ? 32 : 16;
@@ -305,9 +290,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads<GATHER>(), 1
   uint64_t* tempty = tfull + 2;      // [2] accumulator set drained by both CTAs (used in the even CTA)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint32_t* gather_rows = reinterpret_cast<uint32_t*>(smem + STAGES * STAGE_BYTES + 256);  // [GATHER_WARPS][NMAX / 2]
   Experts ex;
-  ex.first_tile = reinterpret_cast<int32_t*>(gather_rows + GATHER_WARPS * (NMAX / 2));  // [E + 1]
+  ex.first_tile = reinterpret_cast<int32_t*>(smem + STAGES * STAGE_BYTES + 256);  // [E + 1]
   ex.begin = ex.first_tile + kMaxExperts + 1;
   ex.end = ex.begin + kMaxExperts + 1;
 
@@ -321,7 +305,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads<GATHER>(), 1
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1 + (GATHER ? 2 : 0));  // expect_tx; a gather warp of each CTA
+      mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -375,8 +359,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads<GATHER>(), 1
   const uint32_t tmem = *tmem_slot;
   const int tiles = ex.first_tile[E] * ct;  // below 2^31: checked by the host for any offsets
 
-  if (warp >= EPI_WARP0 && warp < EPI_WARP0 + EPI_WARPS) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(regs_drain<GATHER>()));
+  if (warp >= EPI_WARP0) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_DRAIN));
     // TMEM lane quarter warp % 4 (channels); every other 32 of the tile's columns (rows)
     typedef typename std::conditional<I8, int32_t, float>::type Sum;
     const int qw = warp & 3, part = (warp - EPI_WARP0) >> 2;
@@ -454,17 +438,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads<GATHER>(), 1
         store_from_f32(a.Y, (first + i / I) * a.ldy + i % I, 0.0f, a.out_dtype);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(regs_few<GATHER>()));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
     if (warp == 0 && lane == 0) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
-      if (!GATHER)
-        for (int b = 0; b < X_MAPS; ++b)
-          asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&xmaps.box[b])) : "memory");
+      for (int b = 0; b < X_MAPS; ++b)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&xmaps.box[b])) : "memory");
       Ring ring;
       bool ok = true, lapped = false;
       for (int q = pair; q < tiles && ok; q += pairs) {
         const Tile t = tile_of(q, ex, E, ct, STEP);
-        const int half = t.n / 2, x_rows = GATHER ? 0 : (half + 15) / 16 * 16;  // <= 128
+        const int half = t.n / 2, x_rows = (half + 15) / 16 * 16;  // <= 128
         const uint32_t bytes = A_BYTES + uint32_t(x_rows) * 128;
         const int ch = (t.block * 2 + int(rank)) * (GLU ? 64 : 128), y = int(t.row0) + int(rank) * half;
         for (int kt = 0; kt < KT; ++kt) {
@@ -526,51 +509,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads<GATHER>(), 1
           if (ok) commit(&tfull[buf]);
         }
       }
-    } else if (GATHER && warp != 0 && warp != 1) {
-      // Gather warp w copies the rows of stage w, whole, and hands it over when they have
-      // landed: about 2 us from a free stage to a full one, in which the tensor core works
-      // on the other five (four warps: a third slower).
-      constexpr uint32_t kNone = 0xFFFFFFFFu;
-      const int w = warp < EPI_WARP0 ? warp - 2 : warp - (EPI_WARP0 + EPI_WARPS) + 2, chunk16 = lane & 7, r_lane = lane >> 3;
-      uint32_t* source = gather_rows + w * (NMAX / 2);  // this CTA's rows of the tile: X offset / 16, kNone: zeros
-      const int64_t kbytes = a.K * (I8 ? 1 : 2);
-      const uint32_t ld16 = uint32_t(a.ldx >> 4);
-      const uint32_t swz0 = uint32_t(chunk16 ^ r_lane) << 4, swz1 = uint32_t(chunk16 ^ (r_lane + 4)) << 4;
-      Ring ring;
-      bool ok = true;
-      for (int q = pair; q < tiles && ok; q += pairs) {
-        const Tile t = tile_of(q, ex, E, ct, STEP);
-        const int half = t.n / 2;  // a multiple of 8
-        __syncwarp();
-        for (int r = lane; r < half; r += 32) {
-          const int p = int(rank) * half + r;
-          const int64_t x = p < t.rows ? source_row(a, t.row0 + p) : -1;
-          source[r] = x >= 0 ? uint32_t(x) * ld16 : kNone;
-        }
-        __syncwarp();
-        for (int kt = 0; kt < KT; ++kt, ring.step()) {
-          const int s = ring.stage;
-          if (s != w) continue;
-          if (!mbar_wait(&empty[s], ring.phase ^ 1, abort_flag, a.status)) {
-            ok = false;
-            break;
-          }
-          const uint32_t dst = smem_u32(smem + s * STAGE_BYTES + A_BYTES) + r_lane * 128;
-          const bool in = kt * 128 + chunk16 * 16 < kbytes;
-          const uint8_t* x = a.X + kt * 128 + chunk16 * 16;
-#pragma unroll 4
-          for (int r = 0; r < half; r += 8) {  // 8 lanes per row: 128 contiguous bytes
-            const uint32_t s0 = source[r + r_lane], s1 = source[r + r_lane + 4];
-            const bool on0 = in && s0 != kNone, on1 = in && s1 != kNone;
-            cp_async16(dst + r * 128 + swz0, on0 ? x + uint64_t(s0) * 16 : a.X, on0);
-            cp_async16(dst + r * 128 + 512 + swz1, on1 ? x + uint64_t(s1) * 16 : a.X, on1);
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads what was copied
-          __syncwarp();
-          if (lane == 0) arrive_even(&full[s]);
-        }
-      }
     }
   }
   tc_fence_before();
@@ -603,24 +541,42 @@ int encode(CUtensorMap* map, const void* base, Kind kind, int rank, const cuuint
   return GQ_OK;
 }
 
-template <bool I8, bool GLU, bool GATHER>
+template <bool I8, bool GLU>
 int launch(const CUtensorMap& wmap, const XMaps& xmaps, const Args& a, Kind kind, unsigned grid, cudaStream_t s) {
-  auto* k = tc_kernel<I8, GLU, GATHER>;
+  auto* k = tc_kernel<I8, GLU>;
   GQ_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_BYTES)));
-  k<<<grid, threads<GATHER>(), SMEM_BYTES, s>>>(wmap, xmaps, a, kind);
+  k<<<grid, THREADS, SMEM_BYTES, s>>>(wmap, xmaps, a, kind);
   return check_launch("tc_kernel");
 }
 
-template <bool I8, bool GLU>
-int launch_gather(const CUtensorMap& wmap, const XMaps& xmaps, const Args& a, Kind kind, unsigned grid,
-                  cudaStream_t s) {
-  return a.rows ? launch<I8, GLU, true>(wmap, xmaps, a, kind, grid, s)
-                : launch<I8, GLU, false>(wmap, xmaps, a, kind, grid, s);
+// dst[s] = X[rows[s]] for the rows of every expert (a row of zeros where there is none).
+// HBM-bound copy: a warp per row, four 16-byte loads per lane in flight.
+__global__ void __launch_bounds__(256) gather_kernel(const Args a, uint4* __restrict__ dst, int64_t vecs) {
+  const int lane = threadIdx.x & 31;
+  const int64_t last = rows_end(a), stride = int64_t(gridDim.x) * (blockDim.x >> 5);
+  for (int64_t s = int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); s < last; s += stride) {
+    const int64_t src = source_row(a, s);
+    const uint4* x = reinterpret_cast<const uint4*>(a.X + (src >= 0 ? src : 0) * a.ldx);
+    for (int64_t v0 = lane; v0 < vecs; v0 += 128) {
+      uint4 r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        r[i] = make_uint4(0, 0, 0, 0);
+        if (src >= 0 && v0 + 32 * i < vecs) r[i] = x[v0 + 32 * i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v0 + 32 * i < vecs) dst[s * vecs + v0 + 32 * i] = r[i];
+    }
+  }
 }
 
 }  // namespace
 
-int launch_tc(const Args& a, Kind kind, bool glu, cudaStream_t s) {
+int launch_tc(const Args& a, Kind kind, bool glu, void* gathered, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  GQ_CUDA_TRY(cudaGetDevice(&dev));
+  GQ_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const cuuint64_t es = kind == S8 ? 1 : 2;
   const cuuint32_t kbox = cuuint32_t(128 / es);
   CUtensorMap wmap;
@@ -633,28 +589,27 @@ int launch_tc(const Args& a, Kind kind, bool glu, cudaStream_t s) {
   const cuuint32_t wbox[4] = {kbox, cuuint32_t(halves), cuuint32_t(128 / halves), 1};
   int st = encode(&wmap, a.W, kind, 4, wdims, wstrides, wbox);
   if (st != GQ_OK) return st;
-  for (int b = 0; b < X_MAPS; ++b) {
-    xmaps.box[b] = wmap;  // not read with a row list
-    if (a.rows) continue;
-    const cuuint64_t xdims[2] = {cuuint64_t(a.K), cuuint64_t(a.n_src)};
-    const cuuint64_t xstrides[1] = {cuuint64_t(a.ldx)};
-    const cuuint32_t xbox[2] = {kbox, cuuint32_t(128 >> b)};
-    st = encode(&xmaps.box[b], a.X, kind, 2, xdims, xstrides, xbox);
+  const int64_t row_bytes = a.K * int64_t(es);
+  if (a.rows) {
+    const int64_t warps = std::min<int64_t>(a.S, int64_t(sms) * 64);
+    gather_kernel<<<unsigned((warps + 7) / 8), 256, 0, s>>>(a, reinterpret_cast<uint4*>(gathered), row_bytes / 16);
+    st = check_launch("gather_kernel");
     if (st != GQ_OK) return st;
   }
-  int dev = 0, sms = 0;
-  GQ_CUDA_TRY(cudaGetDevice(&dev));
-  GQ_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  for (int b = 0; b < X_MAPS; ++b) {
+    const cuuint64_t xdims[2] = {cuuint64_t(a.K), cuuint64_t(a.rows ? a.S : a.n_src)};
+    const cuuint64_t xstrides[1] = {cuuint64_t(a.rows ? row_bytes : a.ldx)};
+    const cuuint32_t xbox[2] = {kbox, cuuint32_t(128 >> b)};
+    st = encode(&xmaps.box[b], a.rows ? gathered : (const void*)a.X, kind, 2, xdims, xstrides, xbox);
+    if (st != GQ_OK) return st;
+  }
   const int64_t blocks = (a.N + 255) / 256;
   const int64_t most = blocks * (a.S / NMAX + std::min(a.S, a.E));  // at least the number of tiles
   GQ_REQUIRE(most < (int64_t(1) << 31) - 65536, "product: too many tiles");
-  GQ_REQUIRE(!a.rows || a.n_src * (a.ldx >> 4) < 0xFFFFFFFFll, "product: X of a row list is limited to 64 GB");
   const unsigned grid = unsigned(2 * std::min<int64_t>(std::max(sms / 2, 1), std::max<int64_t>(most, 1)));
   if (kind == S8)
-    return glu ? launch_gather<true, true>(wmap, xmaps, a, kind, grid, s)
-               : launch_gather<true, false>(wmap, xmaps, a, kind, grid, s);
-  return glu ? launch_gather<false, true>(wmap, xmaps, a, kind, grid, s)
-             : launch_gather<false, false>(wmap, xmaps, a, kind, grid, s);
+    return glu ? launch<true, true>(wmap, xmaps, a, kind, grid, s) : launch<true, false>(wmap, xmaps, a, kind, grid, s);
+  return glu ? launch<false, true>(wmap, xmaps, a, kind, grid, s) : launch<false, false>(wmap, xmaps, a, kind, grid, s);
 }
 
 }  // namespace prod

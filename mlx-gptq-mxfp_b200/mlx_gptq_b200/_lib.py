@@ -61,9 +61,10 @@ SIGNATURES = {
     "gq_route_slots_workspace_size": (SZ, [I64, I64, I64]),
     "gq_route_slots": (I32, [P, I32, I64, I64, I64, P, P, P, P, SZ, P]),
     "gq_combine_slots": (I32, [P, I32, I64, I64, P, P, I64, I64, I64, P, I64, P]),
-    "gq_matmul_grouped": (I32, [P, I64, I64, P, I64, P, I64, P, I64, I64, I64, I64, I32, I32, P, I64, I32, I32, P, P]),
+    "gq_matmul_grouped": (I32, [P, I64, I64, P, I64, P, I64, P, I64, I64, I64, I64, I32, I32, P, I64, I32, I32, P, SZ, P, P]),
+    "gq_matmul_workspace_size": (SZ, [I64, I64, I64, I32, I32]),
     "gq_matmul_int8": (I32, [P, P, I64, I64, P, I64, P, I64, P, P, I64, I64, I64, I64, P, I32, I32, P, I32, I64, I32,
-                             I32, P, P]),
+                             I32, P, SZ, P, P]),
     "gq_pack_q": (I32, [P, I64, I64, I32, P, P]),
     "gq_unpack_q": (I32, [P, I64, I64, I32, I64, P, P]),
     "gq_pack_nibbles": (I32, [P, I64, I64, P, P]),

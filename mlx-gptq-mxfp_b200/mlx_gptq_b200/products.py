@@ -106,6 +106,12 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _workspace(idx, S: int, E: int, w: torch.Tensor, engine: int) -> tuple[torch.Tensor | None, int]:
+    """Where the rows of a row list are gathered, when the kernel that runs wants them so."""
+    n = 0 if idx is None else L.lib().gq_matmul_workspace_size(S, E, w.shape[-1], w.element_size(), engine)
+    return (torch.empty(n, dtype=torch.uint8, device=w.device) if n else None), n
+
+
 def _channels(w: torch.Tensor, glu: bool) -> int:
     if glu and w.shape[-2] % 2:
         raise ValueError(f"glu needs an even number of channels (gate, then up), not {w.shape[-2]}")
@@ -200,11 +206,13 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
         raise ValueError("rows of an empty x")
     xo, ldx, _ = _operand(x)
     wo, ldw, stride_w = _operand(w)
+    eng = _engine(engine)
+    ws, ws_bytes = _workspace(idx, S, E, wo, eng)
     with _on(dev):
         L.check(L.lib().gq_matmul_grouped(L.ptr(xo), xo.shape[0], ldx, L.ptr(idx), S, L.ptr(off), E, L.ptr(wo), N,
                                           wo.shape[-1], ldw, stride_w, L.DTYPE_CODE[x.dtype], int(glu), L.ptr(y),
-                                          _ld(y), int(out is None), _engine(engine), L.ptr(_status(dev)),
-                                          L.stream_ptr(dev)), "matmul_grouped")
+                                          _ld(y), int(out is None), eng, L.ptr(ws), ws_bytes,
+                                          L.ptr(_status(dev)), L.stream_ptr(dev)), "matmul_grouped")
     return y
 
 
@@ -272,11 +280,13 @@ def _int8(xq, xs, wq, ws, offsets, rows, bias, glu, out_dtype, out, engine, what
         raise ValueError("rows of an empty xq")
     xo, ldx, _ = _operand(xq)
     wo, ldw, stride_w = _operand(wq)
+    eng = _engine(engine)
+    ws_, ws_bytes = _workspace(idx, S, E, wo, eng)
     with _on(dev):
         L.check(L.lib().gq_matmul_int8(L.ptr(xo), L.ptr(xs), xo.shape[0], ldx, L.ptr(idx), S, L.ptr(off), E,
                                        L.ptr(wo), L.ptr(ws), N, wo.shape[-1], ldw, stride_w, L.ptr(bias),
                                        0 if bias is None else L.DTYPE_CODE[bias.dtype], int(glu), L.ptr(y),
-                                       L.DTYPE_CODE[out_dtype], _ld(y), int(out is None), _engine(engine),
+                                       L.DTYPE_CODE[out_dtype], _ld(y), int(out is None), eng, L.ptr(ws_), ws_bytes,
                                        L.ptr(_status(dev)), L.stream_ptr(dev)), what)
     return y
 

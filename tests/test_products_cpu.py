@@ -21,20 +21,20 @@ P16 = ctypes.c_void_p(16)
 def _grouped(L, n=4, ldx=16, S=4, E=2, N=8, K=16, ldw=16, stride_w=128, dtype=1, glu=0, ldy=8, engine=-1, offsets=P16,
              rows=None, X=P16, W=P16, Y=P16):
     return L.lib().gq_matmul_grouped(X, n, ldx, rows, S, offsets, E, W, N, K, ldw, stride_w, dtype, glu, Y, ldy, 1,
-                                     engine, None, None)
+                                     engine, None, 0, None, None)
 
 
 def _int8(L, n=4, ldx=16, S=4, E=1, N=8, K=16, ldw=16, stride_w=128, bias=None, glu=0, out=1, ldy=8, offsets=None,
           xs=P16):
     return L.lib().gq_matmul_int8(P16, xs, n, ldx, None, S, offsets, E, P16, P16, N, K, ldw, stride_w, bias, 0, glu,
-                                  P16, out, ldy, 1, -1, None, None)
+                                  P16, out, ldy, 1, -1, None, 0, None, None)
 
 
 @pytest.mark.parametrize("kw", [
     dict(dtype=0), dict(S=-1), dict(S=2 ** 31), dict(E=0), dict(E=1025), dict(N=0), dict(K=12), dict(ldx=12),
     dict(ldx=8), dict(ldw=20), dict(stride_w=4), dict(stride_w=8), dict(glu=1, N=7), dict(ldy=7), dict(engine=2),
     dict(offsets=None), dict(S=5), dict(X=None), dict(W=None), dict(Y=None), dict(X=ctypes.c_void_p(8)),
-    dict(rows=P16, n=0)])
+    dict(rows=P16, n=0), dict(rows=P16, engine=1)])
 def test_grouped_arguments(L, kw):
     assert _grouped(L, **kw) == L.GQ_ERR_ARG and L.last_error().startswith("gq_matmul_grouped")
 
