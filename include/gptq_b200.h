@@ -339,6 +339,28 @@ int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, co
                    int64_t ldy, int zero_behind, int engine, void* workspace, size_t workspace_bytes, int32_t* status,
                    void* stream);
 
+/* The expert MLP of a routed batch in one call: gq_route_slots, gq_matmul_grouped with
+ * glu, gq_matmul_grouped, gq_combine_slots. out[t] = sum over positions j of
+ * weights[t, j] * down_e(silu(gate_e x_t) * up_e x_t), e = index[t, j].
+ * X: [T, K] of dtype (GQ_BF16 / GQ_F16); gate_up: [E, 2 I, K]; down: [E, N, I];
+ * acts: [T * k, I], the rows between the products in slot order (nullable; rows behind the
+ * last slot are left alone); out: [T, N]. I, K and the strides multiples of 8. The rows
+ * between the products and the rows before the sum are rounded to dtype.
+ * own_acts: 1 when acts will be NULL. */
+size_t gq_expert_mlp_workspace_size(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, int64_t N, int own_acts);
+int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, const void* index, int index_bits,
+                  const float* weights, int64_t k, const void* gate_up, int64_t ld_gate_up, int64_t stride_gate_up,
+                  const void* down, int64_t ld_down, int64_t stride_down, int64_t E, int64_t K, int64_t I, int64_t N,
+                  void* acts, int64_t ld_acts, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                  int32_t* status, void* stream);
+
+/* A linear layer in 8 bits in one call: gq_rtn_int8 on the rows of X [M, K], then
+ * gq_matmul_int8 with Wq (codes [N, K rounded up to 16], zeros behind K) and ws [N]. */
+size_t gq_linear_int8_workspace_size(int64_t M, int64_t K);
+int gq_linear_int8(const void* X, int dtype, int64_t M, int64_t K, int64_t ldx, const int8_t* Wq, const float* ws,
+                   int64_t N, int64_t ldw, const void* bias, int bias_dtype, void* Y, int out_dtype, int64_t ldy,
+                   void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
 /* ------------------------------------------------------------------------
  * Packing (mlx_gptq/packing.py, mlx_gptq/artifacts.py)
  * ------------------------------------------------------------------------ */

@@ -1,6 +1,8 @@
 // Data-free grids and packing: RTN affine / MXFP, dequantization, code packing.
 // HBM-bound elementwise work; warps own whole groups so the group reductions
 // (min/max/err sums, max |w|) stay in registers and shuffles.
+#include <type_traits>
+
 #include "gq_affine_grid.cuh"
 
 namespace gq {
@@ -75,9 +77,9 @@ __global__ void __launch_bounds__(256) rtn_mxfp_kernel(const void* __restrict__ 
 // codes do not depend on how the row is cut. A row of zeros (or one whose scale
 // underflows) has s = 0 and codes 0; a row with an Inf or NaN has a non-finite scale, which
 // every product with the row inherits.
-// HBM-bound: each row is read once and held in registers between its maximum and its
-// codes (rows beyond 8 vectors per thread are read again, from L2). TPR threads share a
-// row: a warp where a warp can hold one and there are rows for every SM, else the CTA.
+// HBM-bound: each row is read once and held in registers (NV vectors of V elements per
+// thread) between its maximum and its codes; rows too long for that are read again, from
+// L2. TPR threads share a row.
 // --------------------------------------------------------------------------
 template <typename T, int V>
 __device__ __forceinline__ void load_row_vec(const T* p, float (&v)[V]) {
@@ -109,11 +111,10 @@ __device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[V], floa
   }
 }
 
-template <typename T, int V, int TPR>
+template <typename T, int V, int TPR, int NV>
 __global__ void __launch_bounds__(256) rtn_int8_kernel(const T* __restrict__ X, int64_t rows, int64_t C, int64_t ldx,
                                                        int8_t* __restrict__ q, int64_t Cq, int64_t ldq,
                                                        float* __restrict__ scales) {
-  constexpr int NV = 8;  // vectors a thread holds
   __shared__ uint32_t warp_max_bits[8];
   const int sub = threadIdx.x % TPR;
   const int64_t row = int64_t(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
@@ -137,11 +138,11 @@ __global__ void __launch_bounds__(256) rtn_int8_kernel(const T* __restrict__ X, 
     for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(w[i]) & 0x7FFFFFFFu);
   }
   m = __reduce_max_sync(~0u, m);
-  if constexpr (TPR == 256) {
+  if constexpr (TPR > 32) {
     if ((threadIdx.x & 31) == 0) warp_max_bits[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = max(m, warp_max_bits[w]);
+    for (int w = 0; w < TPR / 32; ++w) m = max(m, warp_max_bits[threadIdx.x / TPR * (TPR / 32) + w]);
   }
   if (!live) return;
   const float s = __uint_as_float(m) / 127.0f;
@@ -167,16 +168,33 @@ int rtn_int8(const void* X, int64_t rows, int64_t C, int64_t ldx, int8_t* q, int
   const T* x = reinterpret_cast<const T*>(X);
   const bool wide = C % 8 == 0 && Cq % 8 == 0 && ldq % 8 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0 && aligned16(X) &&
                     (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
-  const bool by_warp = Cq <= (wide ? 2048 : 256) && rows >= 1184;  // 8 rows for each of 148 SMs
-  const unsigned grid = unsigned(by_warp ? (rows + 7) / 8 : rows);
-  if (wide && by_warp)
-    rtn_int8_kernel<T, 8, 32><<<grid, 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
-  else if (wide)
-    rtn_int8_kernel<T, 8, 256><<<grid, 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
-  else if (by_warp)
-    rtn_int8_kernel<T, 1, 32><<<grid, 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
-  else
-    rtn_int8_kernel<T, 1, 256><<<grid, 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
+  // 8192 rows of 4096 bf16: 2 rows per CTA of 128 threads x 4 vectors.
+  auto run = [&](auto v, auto tpr, auto nv) {
+    constexpr int V = decltype(v)::value, TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+    rtn_int8_kernel<T, V, TPR, NV>
+        <<<unsigned((rows + 256 / TPR - 1) / (256 / TPR)), 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
+  };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, 4> four{};
+  constexpr std::integral_constant<int, 8> eight{};
+  constexpr std::integral_constant<int, 32> warp{};
+  constexpr std::integral_constant<int, 128> half{};
+  constexpr std::integral_constant<int, 256> cta{};
+  if (!wide) {
+    if (Cq <= 256) run(one, warp, eight);
+    else run(one, cta, eight);
+  } else if (Cq <= 512) {
+    run(eight, warp, two);
+  } else if (Cq <= 1024) {
+    run(eight, warp, four);
+  } else if (Cq <= 4096) {
+    run(eight, half, four);
+  } else if (Cq <= 8192) {
+    run(eight, cta, four);
+  } else {
+    run(eight, cta, eight);
+  }
   return check_launch("rtn_int8_kernel");
 }
 

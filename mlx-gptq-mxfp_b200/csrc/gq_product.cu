@@ -87,3 +87,93 @@ extern "C" int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int6
   return run("gq_matmul_int8", a, S8, glu != 0, engine, workspace,
              workspace_bytes, (cudaStream_t)stream);
 }
+
+// ---------------------------------------------------------------------------
+// Runs of them in one call: what a decoding loop calls once per layer, where the host's
+// time per call counts.
+// ---------------------------------------------------------------------------
+namespace {
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct MlpPlan {
+  size_t tok, slot, offsets, route, acts, y, gathered, total;
+};
+
+MlpPlan mlp_plan(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, int64_t N, bool own_acts) {
+  MlpPlan p;
+  const size_t S = size_t(T) * size_t(k);
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  p.tok = take(S * 4);
+  p.slot = take(S * 4);
+  p.offsets = take(size_t(E + 1) * 8);
+  p.route = take(gq_route_slots_workspace_size(T, k, E));
+  p.acts = take(own_acts ? S * size_t(I) * 2 : 0);
+  p.y = take(S * size_t(N) * 2);
+  p.gathered = take(gq_matmul_workspace_size(int64_t(S), E, K, 2, -1));
+  p.total = at;
+  return p;
+}
+
+}  // namespace
+
+extern "C" size_t gq_expert_mlp_workspace_size(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, int64_t N,
+                                               int own_acts) {
+  if (T <= 0 || k <= 0 || T > INT32_MAX / k || E <= 0 || K <= 0 || I <= 0 || N <= 0) return 0;
+  return mlp_plan(T, k, E, K, I, N, own_acts != 0).total;
+}
+
+extern "C" int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, const void* index, int index_bits,
+                             const float* weights, int64_t k, const void* gate_up, int64_t ld_gate_up,
+                             int64_t stride_gate_up, const void* down, int64_t ld_down, int64_t stride_down, int64_t E,
+                             int64_t K, int64_t I, int64_t N, void* acts, int64_t ld_acts, void* out, int64_t ldo,
+                             void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  GQ_REQUIRE(T >= 0 && k >= 1 && T <= INT32_MAX / k && E >= 1 && K >= 1 && I >= 1 && N >= 1, "gq_expert_mlp: sizes");
+  if (T == 0) return GQ_OK;
+  GQ_REQUIRE(index && weights && out, "gq_expert_mlp: null pointer");
+  GQ_REQUIRE(I % 8 == 0 && (!acts || ld_acts % 8 == 0), "gq_expert_mlp: activation rows must be 16-byte aligned");
+  const MlpPlan p = mlp_plan(T, k, E, K, I, N, acts == nullptr);
+  GQ_REQUIRE(workspace && workspace_bytes >= p.total && aligned16(workspace),
+             "gq_expert_mlp: workspace too small (%zu < %zu)", workspace_bytes, p.total);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  int32_t *tok = reinterpret_cast<int32_t*>(ws + p.tok), *slot = reinterpret_cast<int32_t*>(ws + p.slot);
+  int64_t* offsets = reinterpret_cast<int64_t*>(ws + p.offsets);
+  const int64_t S = T * k;
+  if (!acts) acts = ws + p.acts, ld_acts = I;
+  int st = gq_route_slots(index, index_bits, T, k, E, tok, slot, offsets, ws + p.route, p.acts - p.route, stream);
+  if (st != GQ_OK) return st;
+  st = gq_matmul_grouped(X, T, ldx, tok, S, offsets, E, gate_up, 2 * I, K, ld_gate_up, stride_gate_up, dtype, 1, acts,
+                         ld_acts, 0, -1, ws + p.gathered, p.total - p.gathered, status, stream);
+  if (st != GQ_OK) return st;
+  st = gq_matmul_grouped(acts, S, ld_acts, nullptr, S, offsets, E, down, N, I, ld_down, stride_down, dtype, 0, ws + p.y,
+                         N, 0, -1, nullptr, 0, status, stream);
+  if (st != GQ_OK) return st;
+  return gq_combine_slots(ws + p.y, dtype, S, N, slot, weights, T, k, N, out, ldo, stream);
+}
+
+extern "C" size_t gq_linear_int8_workspace_size(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return 0;
+  return align256(size_t(M) * 4) + size_t(M) * size_t((K + 15) / 16 * 16);
+}
+
+extern "C" int gq_linear_int8(const void* X, int dtype, int64_t M, int64_t K, int64_t ldx, const int8_t* Wq,
+                              const float* ws, int64_t N, int64_t ldw, const void* bias, int bias_dtype, void* Y,
+                              int out_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, int32_t* status,
+                              void* stream) {
+  if (M == 0) return GQ_OK;
+  const size_t need = gq_linear_int8_workspace_size(M, K);
+  GQ_REQUIRE(need && workspace && workspace_bytes >= need && aligned16(workspace),
+             "gq_linear_int8: workspace too small (%zu < %zu)", workspace_bytes, need);
+  const int64_t Kp = (K + 15) / 16 * 16;
+  float* xs = reinterpret_cast<float*>(workspace);
+  int8_t* q = reinterpret_cast<int8_t*>(workspace) + align256(size_t(M) * 4);
+  const int st = gq_rtn_int8(X, dtype, M, K, ldx, q, Kp, Kp, xs, stream);
+  if (st != GQ_OK) return st;
+  return gq_matmul_int8(q, xs, M, Kp, nullptr, M, nullptr, 1, Wq, ws, N, Kp, ldw, N * ldw, bias, bias_dtype, 0, Y,
+                        out_dtype, ldy, 0, -1, nullptr, 0, status, stream);
+}

@@ -19,7 +19,7 @@ namespace prod {
 namespace {
 
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
-constexpr int UNROLL = 4;  // 64-byte blocks in flight per warp
+constexpr int UNROLL = 4;  // 64-byte blocks of each channel in flight per warp
 
 __device__ __forceinline__ uint4 load16(const uint8_t* p, bool on) {
   uint4 v = make_uint4(0, 0, 0, 0);
@@ -57,9 +57,11 @@ __device__ __forceinline__ void mma(T (&c)[4], uint32_t a0, uint32_t a1, uint32_
 }
 
 // blockIdx.y: the expert, or with by_row (fewer rows than experts) a product row, which
-// stands for the expert that begins there; the last y writes the rows behind.
+// stands for the expert that begins there; one more y, where there is one, writes the rows
+// behind. The weights wait for the expert, so it is found in one step of memory latency:
+// every lane of a warp counts the offsets at or before the row.
 template <int KIND, bool GLU, int NT>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int by_row) {
+__global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int by_row, const int experts_y) {
   typedef typename Acc<KIND>::T T;
   __shared__ T part[WARPS][NT][4][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -67,25 +69,20 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int b
   constexpr int CH = GLU ? 8 : 16;        // of them per CTA
   const int64_t c0 = int64_t(blockIdx.x) * CH;
 
-  if (blockIdx.y == gridDim.y - 1) {
-    if (a.zero_behind) {
-      for (int64_t s = rows_end(a) + threadIdx.x / CH; s < a.S; s += THREADS / CH) {
-        const int64_t c = c0 + threadIdx.x % CH;
-        if (c < I) store_from_f32(a.Y, s * a.ldy + c, 0.0f, a.out_dtype);
-      }
+  if (int(blockIdx.y) == experts_y) {
+    for (int64_t s = rows_end(a) + threadIdx.x / CH; s < a.S; s += THREADS / CH) {
+      const int64_t c = c0 + threadIdx.x % CH;
+      if (c < I) store_from_f32(a.Y, s * a.ldy + c, 0.0f, a.out_dtype);
     }
     return;
   }
-  int64_t e = blockIdx.y;
+  int64_t e = blockIdx.y, begin, end;
   if (by_row) {
-    int64_t lo = 0, hi = a.E;  // last expert with offsets[e] <= row
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.offsets[mid] <= int64_t(blockIdx.y)) lo = mid; else hi = mid;
-    }
-    e = lo;
+    int before = 0;  // offsets[0 .. E - 1] at or before the row: the last of them begins its expert
+    for (int64_t i = lane; i < a.E; i += 32) before += a.offsets[i] <= int64_t(blockIdx.y);
+    e = __reduce_add_sync(~0u, before) - 1;
+    if (e < 0) return;
   }
-  int64_t begin, end;
   segment(a, e, begin, end);
   if (begin >= end || (by_row && begin != int64_t(blockIdx.y))) return;
 
@@ -167,15 +164,15 @@ template <int KIND, bool GLU>
 int launch_nt(const Args& a, cudaStream_t s) {
   const int64_t I = GLU ? a.N / 2 : a.N, CH = GLU ? 8 : 16;
   const int by_row = a.offsets && a.S < a.E;
-  const int64_t gx = (I + CH - 1) / CH, gy = (by_row ? a.S : a.E) + 1;
-  const dim3 grid{unsigned(gx), unsigned(gy)};
+  const int64_t gx = (I + CH - 1) / CH, experts = by_row ? a.S : a.E;
+  const dim3 grid{unsigned(gx), unsigned(experts + (a.zero_behind && a.offsets ? 1 : 0))};
   const int64_t most = a.offsets ? (a.S + a.E - 1) / a.E * 2 : a.S;  // rows of a busy expert
   if (most <= 8)
-    rows_kernel<KIND, GLU, 1><<<grid, THREADS, 0, s>>>(a, by_row);
+    rows_kernel<KIND, GLU, 1><<<grid, THREADS, 0, s>>>(a, by_row, int(experts));
   else if (most <= 16)
-    rows_kernel<KIND, GLU, 2><<<grid, THREADS, 0, s>>>(a, by_row);
+    rows_kernel<KIND, GLU, 2><<<grid, THREADS, 0, s>>>(a, by_row, int(experts));
   else
-    rows_kernel<KIND, GLU, 4><<<grid, THREADS, 0, s>>>(a, by_row);
+    rows_kernel<KIND, GLU, 4><<<grid, THREADS, 0, s>>>(a, by_row, int(experts));
   return check_launch("rows_kernel");
 }
 

@@ -65,6 +65,11 @@ SIGNATURES = {
     "gq_matmul_workspace_size": (SZ, [I64, I64, I64, I32, I32]),
     "gq_matmul_int8": (I32, [P, P, I64, I64, P, I64, P, I64, P, P, I64, I64, I64, I64, P, I32, I32, P, I32, I64, I32,
                              I32, P, SZ, P, P]),
+    "gq_expert_mlp_workspace_size": (SZ, [I64, I64, I64, I64, I64, I64, I32]),
+    "gq_expert_mlp": (I32, [P, I32, I64, I64, P, I32, P, I64, P, I64, I64, P, I64, I64, I64, I64, I64, I64, P, I64, P,
+                            I64, P, SZ, P, P]),
+    "gq_linear_int8_workspace_size": (SZ, [I64, I64]),
+    "gq_linear_int8": (I32, [P, I32, I64, I64, I64, P, P, I64, I64, P, I32, P, I32, I64, P, SZ, P, P]),
     "gq_pack_q": (I32, [P, I64, I64, I32, P, P]),
     "gq_unpack_q": (I32, [P, I64, I64, I32, I64, P, P]),
     "gq_pack_nibbles": (I32, [P, I64, I64, P, P]),

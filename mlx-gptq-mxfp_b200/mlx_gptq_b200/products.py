@@ -21,6 +21,7 @@ They have no backward: with gradients enabled, inputs that require them are refu
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 
@@ -33,21 +34,43 @@ ENGINES = {None: -1, "rows": 0, "tcgen05": 1}
 def _forward_only(what: str, *tensors) -> torch.device:
     """The tensors' common CUDA device; refuses a call that autograd would have to follow."""
     dev = L.require_cuda(*tensors)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
     return dev
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(dev: torch.device):
     """Launches go to `dev`, whatever device is current."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
-def _status(dev: torch.device) -> torch.Tensor:
+def _stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _status(dev: torch.device) -> int:
     """The device's status word; its first use allocates it, which must not be captured."""
-    if torch.cuda.is_current_stream_capturing() and dev.index not in L._status_words:
-        raise RuntimeError("make one call on this device before capturing a CUDA graph")
-    return L.status_word(dev)
+    word = L._status_words.get(dev.index)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("make one call on this device before capturing a CUDA graph")
+        word = L.status_word(dev)
+    return word.data_ptr()
+
+
+# Workspace sizes are functions of the sizes alone; asking the library costs a call each.
+@functools.lru_cache(4096)
+def _size(name: str, *sizes: int) -> int:
+    return getattr(L.lib(), name)(*sizes)
+
+
+def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
 def _engine(engine) -> int:
@@ -106,10 +129,10 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _workspace(idx, S: int, E: int, w: torch.Tensor, engine: int) -> tuple[torch.Tensor | None, int]:
+def _gathered(idx, S: int, E: int, w: torch.Tensor, engine: int) -> tuple[torch.Tensor | None, int]:
     """Where the rows of a row list are gathered, when the kernel that runs wants them so."""
-    n = 0 if idx is None else L.lib().gq_matmul_workspace_size(S, E, w.shape[-1], w.element_size(), engine)
-    return (torch.empty(n, dtype=torch.uint8, device=w.device) if n else None), n
+    n = 0 if idx is None else _size("gq_matmul_workspace_size", S, E, w.shape[-1], w.element_size(), engine)
+    return _scratch(n, w.device), n
 
 
 def _channels(w: torch.Tensor, glu: bool) -> int:
@@ -146,12 +169,11 @@ def route_slots(top_k_index: torch.Tensor, num_experts: int) -> tuple[torch.Tens
     tok = torch.empty(T * k, dtype=torch.int32, device=dev)
     slot = torch.empty(T, k, dtype=torch.int32, device=dev)
     offsets = torch.empty(num_experts + 1, dtype=torch.int64, device=dev)
-    lib = L.lib()
-    ws_bytes = lib.gq_route_slots_workspace_size(T, k, num_experts)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    ws_bytes = _size("gq_route_slots_workspace_size", T, k, num_experts)
+    ws = _scratch(ws_bytes, dev)
     with _on(dev):
-        L.check(lib.gq_route_slots(L.ptr(idx), 8 * idx.element_size(), T, k, num_experts, L.ptr(tok), L.ptr(slot),
-                                   L.ptr(offsets), L.ptr(ws), ws_bytes, L.stream_ptr(dev)), "route_slots")
+        L.check(L.lib().gq_route_slots(L.ptr(idx), 8 * idx.element_size(), T, k, num_experts, L.ptr(tok), L.ptr(slot),
+                                       L.ptr(offsets), L.ptr(ws), ws_bytes, _stream(dev)), "route_slots")
     return tok, slot, offsets
 
 
@@ -176,7 +198,7 @@ def combine_slots(y: torch.Tensor, slot: torch.Tensor, weights: torch.Tensor,
     sl, w = slot.contiguous(), weights.to(torch.float32).contiguous()
     with _on(dev):
         L.check(L.lib().gq_combine_slots(L.ptr(y), L.DTYPE_CODE[y.dtype], S, _ld(y), L.ptr(sl), L.ptr(w), T, k, N,
-                                         L.ptr(out), _ld(out), L.stream_ptr(dev)), "combine_slots")
+                                         L.ptr(out), _ld(out), _stream(dev)), "combine_slots")
     return out
 
 
@@ -207,12 +229,12 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     xo, ldx, _ = _operand(x)
     wo, ldw, stride_w = _operand(w)
     eng = _engine(engine)
-    ws, ws_bytes = _workspace(idx, S, E, wo, eng)
+    ws, ws_bytes = _gathered(idx, S, E, wo, eng)
     with _on(dev):
         L.check(L.lib().gq_matmul_grouped(L.ptr(xo), xo.shape[0], ldx, L.ptr(idx), S, L.ptr(off), E, L.ptr(wo), N,
                                           wo.shape[-1], ldw, stride_w, L.DTYPE_CODE[x.dtype], int(glu), L.ptr(y),
                                           _ld(y), int(out is None), eng, L.ptr(ws), ws_bytes,
-                                          L.ptr(_status(dev)), L.stream_ptr(dev)), "matmul_grouped")
+                                          _status(dev), _stream(dev)), "matmul_grouped")
     return y
 
 
@@ -235,21 +257,51 @@ def expert_mlp(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.
         raise ValueError("top_k_index and top_k_weights must be [tokens, k]")
     T, k = top_k_index.shape
     I = down.shape[2]
-    acts = _output(acts, (T * k, I), x.dtype, dev, "acts")
-    out = _output(out, (T, down.shape[1]), x.dtype, dev)
+    if not top_k_weights.is_floating_point():
+        raise ValueError("top_k_weights must be floating point")
+    if top_k_index.dtype not in (torch.int32, torch.int64) or k == 0:
+        raise ValueError("top_k_index must be int32 or int64 [tokens, k]")
+    for w in (gate_up, down):
+        if x.dtype != w.dtype or x.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"rows and weights must all be bf16 or f16, not {x.dtype} and {w.dtype}")
+    E, N = down.shape[:2]
+    if acts is not None:
+        acts = _output(acts, (T * k, I), x.dtype, dev, "acts")
+    out = _output(out, (T, N), x.dtype, dev)
     if T == 0:
         return out
-    tok, slot, offsets = route_slots(top_k_index, gate_up.shape[0])
-    matmul_grouped(x, gate_up, offsets, rows=tok, glu=True, out=acts)
-    y = torch.empty(T * k, down.shape[1], dtype=x.dtype, device=dev)
-    matmul_grouped(acts, down, offsets, out=y)
-    return combine_slots(y, slot, top_k_weights, out=out)
+    if I % 8 or (acts is not None and (_ld(acts) % 8 or acts.data_ptr() % 16)):
+        # activation rows that the second product cannot read in place
+        tok, slot, offsets = route_slots(top_k_index, E)
+        h = matmul_grouped(x, gate_up, offsets, rows=tok, glu=True, out=acts)
+        y = matmul_grouped(h, down, offsets)
+        return combine_slots(y, slot, top_k_weights, out=out)
+    xo, ldx, _ = _operand(x)
+    gu, ld_gu, stride_gu = _operand(gate_up)
+    dn, ld_dn, stride_dn = _operand(down)
+    idx, wt = top_k_index.contiguous(), top_k_weights.to(torch.float32).contiguous()
+    K = gu.shape[2]
+    nbytes = _size("gq_expert_mlp_workspace_size", T, k, E, K, I, N, int(acts is None))
+    ws = _scratch(nbytes, dev)
+    with _on(dev):
+        L.check(L.lib().gq_expert_mlp(
+            xo.data_ptr(), L.DTYPE_CODE[x.dtype], T, ldx, idx.data_ptr(), 8 * idx.element_size(), wt.data_ptr(), k,
+            gu.data_ptr(), ld_gu, stride_gu, dn.data_ptr(), ld_dn, stride_dn, E, K, I, N, L.ptr(acts),
+            0 if acts is None else _ld(acts), out.data_ptr(), _ld(out), ws.data_ptr(), nbytes, _status(dev),
+            _stream(dev)), "expert_mlp")
+    return out
 
 
 def _scales(s: torch.Tensor, shape, name: str) -> torch.Tensor:
     if s.dtype != torch.float32 or tuple(s.shape) != tuple(shape):
         raise ValueError(f"{name} must be float32 {list(shape)}")
     return s.contiguous()
+
+
+def _check_bias(bias: torch.Tensor, N: int) -> torch.Tensor:
+    if bias.shape != (N,) or bias.dtype not in L.DTYPE_CODE:
+        raise ValueError(f"bias must be floating point [{N}]")
+    return bias.contiguous()
 
 
 def _int8(xq, xs, wq, ws, offsets, rows, bias, glu, out_dtype, out, engine, what):
@@ -270,9 +322,7 @@ def _int8(xq, xs, wq, ws, offsets, rows, bias, glu, out_dtype, out, engine, what
     idx = _row_list(rows, xq.shape[0])
     S = xq.shape[0] if idx is None else idx.shape[0]
     if bias is not None:
-        if bias.shape != (N,) or bias.dtype not in L.DTYPE_CODE:
-            raise ValueError(f"bias must be floating point [{N}]")
-        bias = bias.contiguous()
+        bias = _check_bias(bias, N)
     y = _output(out, (S, _channels(wq, glu)), out_dtype, dev)
     if S == 0:
         return y
@@ -281,13 +331,13 @@ def _int8(xq, xs, wq, ws, offsets, rows, bias, glu, out_dtype, out, engine, what
     xo, ldx, _ = _operand(xq)
     wo, ldw, stride_w = _operand(wq)
     eng = _engine(engine)
-    ws_, ws_bytes = _workspace(idx, S, E, wo, eng)
+    ws_, ws_bytes = _gathered(idx, S, E, wo, eng)
     with _on(dev):
         L.check(L.lib().gq_matmul_int8(L.ptr(xo), L.ptr(xs), xo.shape[0], ldx, L.ptr(idx), S, L.ptr(off), E,
                                        L.ptr(wo), L.ptr(ws), N, wo.shape[-1], ldw, stride_w, L.ptr(bias),
                                        0 if bias is None else L.DTYPE_CODE[bias.dtype], int(glu), L.ptr(y),
                                        L.DTYPE_CODE[out_dtype], _ld(y), int(out is None), eng, L.ptr(ws_), ws_bytes,
-                                       L.ptr(_status(dev)), L.stream_ptr(dev)), what)
+                                       _status(dev), _stream(dev)), what)
     return y
 
 
@@ -316,15 +366,32 @@ def linear_int8(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias: torch
     """A linear layer in 8 bits: the rows of x [..., K] (bf16, f16 or f32) quantized to int8
     with one scale per row (grid.rtn_quantize_int8), times wq [N, K] / ws [N] quantized the
     same way, + bias. Returns [..., N] in out_dtype (default: x's)."""
-    from .grid import _int8_codes
-
     dev = _forward_only("linear_int8", x, wq, ws, bias)
-    if x.dim() < 1 or wq.dim() != 2 or x.shape[-1] != wq.shape[1] or wq.shape[1] == 0:
+    if x.dim() < 1 or wq.dim() != 2 or x.shape[-1] != wq.shape[1] or 0 in wq.shape:
         raise ValueError(f"shapes: x [..., K] {list(x.shape)}, wq [N, K] {list(wq.shape)}")
-    if wq.device != dev:
-        raise RuntimeError("tensors on different devices")
-    K = wq.shape[1]
-    q, s = _int8_codes(x.reshape(-1, K), -(-K // 16) * 16)
-    y = matmul_int8(q[:, :K], s, wq, ws, bias, out_dtype or x.dtype) if K % 16 == 0 else \
-        matmul_int8(q, s, _operand(wq)[0], ws, bias, out_dtype or x.dtype)
-    return y.reshape(*x.shape[:-1], wq.shape[0])
+    out_dtype = out_dtype or x.dtype
+    if x.dtype not in L.DTYPE_CODE or out_dtype not in L.DTYPE_CODE:
+        raise ValueError(f"unsupported dtype {x.dtype} or {out_dtype}")
+    if wq.dtype != torch.int8:
+        raise ValueError(f"codes must be int8, not {wq.dtype}")
+    N, K = wq.shape
+    if K > 131071:
+        raise ValueError(f"K = {K}: sums of 8-bit products fit 32 bits up to 131071")
+    ws = _scales(ws, (N,), "ws")
+    if bias is not None:
+        bias = _check_bias(bias, N)
+    rows = x.reshape(-1, K)
+    M = rows.shape[0]
+    y = torch.empty(M, N, dtype=out_dtype, device=dev)
+    if M:
+        if (K > 1 and rows.stride(1) != 1) or (M > 1 and rows.stride(0) < K):
+            rows = rows.contiguous()
+        wo, ldw, _ = _operand(wq)
+        nbytes = _size("gq_linear_int8_workspace_size", M, K)
+        scratch = _scratch(nbytes, dev)
+        with _on(dev):
+            L.check(L.lib().gq_linear_int8(
+                rows.data_ptr(), L.DTYPE_CODE[x.dtype], M, K, _ld(rows), wo.data_ptr(), ws.data_ptr(), N, ldw,
+                L.ptr(bias), 0 if bias is None else L.DTYPE_CODE[bias.dtype], y.data_ptr(), L.DTYPE_CODE[out_dtype], N,
+                scratch.data_ptr(), nbytes, _status(dev), _stream(dev)), "linear_int8")
+    return y.reshape(*x.shape[:-1], N)
