@@ -46,6 +46,31 @@ EncodeTiledFn tensor_map_encoder();
     }                                                                            \
   } while (0)
 
+// Launch that may begin while the kernel before it in the stream ends (programmatic
+// dependent launch): the kernel calls grid_wait() before it touches what earlier kernels
+// write, and grid_release() once it has (see there).
+template <typename... P, typename... A>
+int launch_dependent(const char* what, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
+                     A... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, P(args)...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_last_error("%s: %s", what, cudaGetErrorString(e));
+    return GQ_ERR_CUDA;
+  }
+  return GQ_OK;
+}
+
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---------------------------------------------------------------------------
@@ -306,6 +331,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     }
   }
 }
+
+// Waits until every kernel before this one in the stream has completed and its writes are
+// visible. Every thread that reads or writes global memory calls it first (or is ordered
+// after a thread that did).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next kernel (if launched with launch_dependent) begin. Called after grid_wait(),
+// so a kernel that has begun may already read what kernels before its predecessor wrote.
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
 // TMA and tcgen05 wrappers (inline PTX, sm_100a)

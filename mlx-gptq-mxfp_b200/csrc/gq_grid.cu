@@ -116,6 +116,8 @@ __global__ void __launch_bounds__(256) rtn_int8_kernel(const T* __restrict__ X, 
                                                        int8_t* __restrict__ q, int64_t Cq, int64_t ldq,
                                                        float* __restrict__ scales) {
   __shared__ uint32_t warp_max_bits[8];
+  grid_wait();
+  grid_release();
   const int sub = threadIdx.x % TPR;
   const int64_t row = int64_t(blockIdx.x) * (256 / TPR) + threadIdx.x / TPR;
   const bool live = row < rows;
@@ -171,8 +173,9 @@ int rtn_int8(const void* X, int64_t rows, int64_t C, int64_t ldx, int8_t* q, int
   // 8192 rows of 4096 bf16: 2 rows per CTA of 128 threads x 4 vectors.
   auto run = [&](auto v, auto tpr, auto nv) {
     constexpr int V = decltype(v)::value, TPR = decltype(tpr)::value, NV = decltype(nv)::value;
-    rtn_int8_kernel<T, V, TPR, NV>
-        <<<unsigned((rows + 256 / TPR - 1) / (256 / TPR)), 256, 0, s>>>(x, rows, C, ldx, q, Cq, ldq, scales);
+    return launch_dependent("rtn_int8_kernel", rtn_int8_kernel<T, V, TPR, NV>,
+                            dim3(unsigned((rows + 256 / TPR - 1) / (256 / TPR))), 256, 0, s, x, rows, C, ldx, q, Cq,
+                            ldq, scales);
   };
   constexpr std::integral_constant<int, 1> one{};
   constexpr std::integral_constant<int, 2> two{};
@@ -181,21 +184,12 @@ int rtn_int8(const void* X, int64_t rows, int64_t C, int64_t ldx, int8_t* q, int
   constexpr std::integral_constant<int, 32> warp{};
   constexpr std::integral_constant<int, 128> half{};
   constexpr std::integral_constant<int, 256> cta{};
-  if (!wide) {
-    if (Cq <= 256) run(one, warp, eight);
-    else run(one, cta, eight);
-  } else if (Cq <= 512) {
-    run(eight, warp, two);
-  } else if (Cq <= 1024) {
-    run(eight, warp, four);
-  } else if (Cq <= 4096) {
-    run(eight, half, four);
-  } else if (Cq <= 8192) {
-    run(eight, cta, four);
-  } else {
-    run(eight, cta, eight);
-  }
-  return check_launch("rtn_int8_kernel");
+  if (!wide) return Cq <= 256 ? run(one, warp, eight) : run(one, cta, eight);
+  if (Cq <= 512) return run(eight, warp, two);
+  if (Cq <= 1024) return run(eight, warp, four);
+  if (Cq <= 4096) return run(eight, half, four);
+  if (Cq <= 8192) return run(eight, cta, four);
+  return run(eight, cta, eight);
 }
 
 // --------------------------------------------------------------------------

@@ -40,37 +40,25 @@ int run(const char* what, const Args& a, Kind kind, bool glu, int engine, void* 
   return launch_tc(a, kind, glu, workspace, s);
 }
 
-}  // namespace
-}  // namespace prod
-}  // namespace gq
-
-using namespace gq;
-using namespace gq::prod;
-
-extern "C" size_t gq_matmul_workspace_size(int64_t S, int64_t E, int64_t K, int element_bytes, int engine) {
-  if (S <= 0 || E <= 0 || K <= 0) return 0;
-  return by_rows(S, E, engine) ? 0 : size_t(S) * size_t(K) * size_t(element_bytes);
-}
-
-extern "C" int gq_matmul_grouped(const void* X, int64_t n, int64_t ldx, const int32_t* rows, int64_t S,
-                                 const int64_t* offsets, int64_t E, const void* W, int64_t N, int64_t K, int64_t ldw,
-                                 int64_t stride_w, int dtype, int glu, void* Y, int64_t ldy, int zero_behind,
-                                 int engine, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+// early (see Args): only for launches that follow one of this library's own kernels.
+int grouped(bool early, const void* X, int64_t n, int64_t ldx, const int32_t* rows, int64_t S, const int64_t* offsets,
+            int64_t E, const void* W, int64_t N, int64_t K, int64_t ldw, int64_t stride_w, int dtype, int glu, void* Y,
+            int64_t ldy, int zero_behind, int engine, void* workspace, size_t workspace_bytes, int32_t* status,
+            void* stream) {
   GQ_REQUIRE(dtype == GQ_BF16 || dtype == GQ_F16, "gq_matmul_grouped: rows and weights are bf16 or f16 (dtype %d)",
              dtype);
   Args a = {};
   a.X = (const uint8_t*)X, a.n_src = n, a.ldx = 2 * ldx, a.rows = rows, a.offsets = offsets, a.E = E, a.S = S;
   a.W = (const uint8_t*)W, a.N = N, a.K = K, a.ldw = 2 * ldw, a.stride_w = 2 * stride_w;
-  a.Y = Y, a.ldy = ldy, a.out_dtype = dtype, a.zero_behind = zero_behind, a.status = status;
-  return run("gq_matmul_grouped", a, dtype == GQ_BF16 ? BF16 : F16, glu != 0, engine, workspace,
-             workspace_bytes, (cudaStream_t)stream);
+  a.Y = Y, a.ldy = ldy, a.out_dtype = dtype, a.zero_behind = zero_behind, a.status = status, a.early = early;
+  return run("gq_matmul_grouped", a, dtype == GQ_BF16 ? BF16 : F16, glu != 0, engine, workspace, workspace_bytes,
+             (cudaStream_t)stream);
 }
 
-extern "C" int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, const int32_t* rows,
-                              int64_t S, const int64_t* offsets, int64_t E, const int8_t* Wq, const float* ws,
-                              int64_t N, int64_t K, int64_t ldw, int64_t stride_w, const void* bias, int bias_dtype,
-                              int glu, void* Y, int out_dtype, int64_t ldy, int zero_behind, int engine,
-                              void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+int int8(bool early, const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, const int32_t* rows, int64_t S,
+         const int64_t* offsets, int64_t E, const int8_t* Wq, const float* ws, int64_t N, int64_t K, int64_t ldw,
+         int64_t stride_w, const void* bias, int bias_dtype, int glu, void* Y, int out_dtype, int64_t ldy,
+         int zero_behind, int engine, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   GQ_REQUIRE(out_dtype == GQ_BF16 || out_dtype == GQ_F16 || out_dtype == GQ_F32, "gq_matmul_int8: out dtype %d",
              out_dtype);
   GQ_REQUIRE(!bias || bias_dtype == GQ_BF16 || bias_dtype == GQ_F16 || bias_dtype == GQ_F32,
@@ -83,9 +71,36 @@ extern "C" int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int6
   a.X = (const uint8_t*)Xq, a.n_src = n, a.ldx = ldx, a.rows = rows, a.offsets = offsets, a.E = E, a.S = S;
   a.W = (const uint8_t*)Wq, a.N = N, a.K = K, a.ldw = ldw, a.stride_w = stride_w;
   a.xs = xs, a.ws = ws, a.bias = bias, a.bias_dtype = bias_dtype;
-  a.Y = Y, a.ldy = ldy, a.out_dtype = out_dtype, a.zero_behind = zero_behind, a.status = status;
-  return run("gq_matmul_int8", a, S8, glu != 0, engine, workspace,
-             workspace_bytes, (cudaStream_t)stream);
+  a.Y = Y, a.ldy = ldy, a.out_dtype = out_dtype, a.zero_behind = zero_behind, a.status = status, a.early = early;
+  return run("gq_matmul_int8", a, S8, glu != 0, engine, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+}  // namespace
+}  // namespace prod
+}  // namespace gq
+
+using namespace gq;
+
+extern "C" size_t gq_matmul_workspace_size(int64_t S, int64_t E, int64_t K, int element_bytes, int engine) {
+  if (S <= 0 || E <= 0 || K <= 0) return 0;
+  return prod::by_rows(S, E, engine) ? 0 : size_t(S) * size_t(K) * size_t(element_bytes);
+}
+
+extern "C" int gq_matmul_grouped(const void* X, int64_t n, int64_t ldx, const int32_t* rows, int64_t S,
+                                 const int64_t* offsets, int64_t E, const void* W, int64_t N, int64_t K, int64_t ldw,
+                                 int64_t stride_w, int dtype, int glu, void* Y, int64_t ldy, int zero_behind,
+                                 int engine, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  return prod::grouped(false, X, n, ldx, rows, S, offsets, E, W, N, K, ldw, stride_w, dtype, glu, Y, ldy, zero_behind,
+                       engine, workspace, workspace_bytes, status, stream);
+}
+
+extern "C" int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, const int32_t* rows,
+                              int64_t S, const int64_t* offsets, int64_t E, const int8_t* Wq, const float* ws,
+                              int64_t N, int64_t K, int64_t ldw, int64_t stride_w, const void* bias, int bias_dtype,
+                              int glu, void* Y, int out_dtype, int64_t ldy, int zero_behind, int engine,
+                              void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  return prod::int8(false, Xq, xs, n, ldx, rows, S, offsets, E, Wq, ws, N, K, ldw, stride_w, bias, bias_dtype, glu, Y,
+                    out_dtype, ldy, zero_behind, engine, workspace, workspace_bytes, status, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -150,7 +165,7 @@ extern "C" int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, c
   st = gq_matmul_grouped(X, T, ldx, tok, S, offsets, E, gate_up, 2 * I, K, ld_gate_up, stride_gate_up, dtype, 1, acts,
                          ld_acts, 0, -1, ws + p.gathered, p.total - p.gathered, status, stream);
   if (st != GQ_OK) return st;
-  st = gq_matmul_grouped(acts, S, ld_acts, nullptr, S, offsets, E, down, N, I, ld_down, stride_down, dtype, 0, ws + p.y,
+  st = prod::grouped(true, acts, S, ld_acts, nullptr, S, offsets, E, down, N, I, ld_down, stride_down, dtype, 0, ws + p.y,
                          N, 0, -1, nullptr, 0, status, stream);
   if (st != GQ_OK) return st;
   return gq_combine_slots(ws + p.y, dtype, S, N, slot, weights, T, k, N, out, ldo, stream);
@@ -174,6 +189,6 @@ extern "C" int gq_linear_int8(const void* X, int dtype, int64_t M, int64_t K, in
   int8_t* q = reinterpret_cast<int8_t*>(workspace) + align256(size_t(M) * 4);
   const int st = gq_rtn_int8(X, dtype, M, K, ldx, q, Kp, Kp, xs, stream);
   if (st != GQ_OK) return st;
-  return gq_matmul_int8(q, xs, M, Kp, nullptr, M, nullptr, 1, Wq, ws, N, Kp, ldw, N * ldw, bias, bias_dtype, 0, Y,
+  return prod::int8(true, q, xs, M, Kp, nullptr, M, nullptr, 1, Wq, ws, N, Kp, ldw, N * ldw, bias, bias_dtype, 0, Y,
                         out_dtype, ldy, 0, -1, nullptr, 0, status, stream);
 }

@@ -32,6 +32,7 @@ struct Args {
   int out_dtype;
   int zero_behind;         // rows behind the last expert's: 1 = written as zeros, 0 = left alone
   int32_t* status;         // nullable
+  int early;               // W and offsets are not written by the kernel launched just before
 };
 
 int launch_rows(const Args& a, Kind kind, bool glu, cudaStream_t s);

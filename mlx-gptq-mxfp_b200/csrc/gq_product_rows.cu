@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int b
   constexpr int CH = GLU ? 8 : 16;        // of them per CTA
   const int64_t c0 = int64_t(blockIdx.x) * CH;
 
+  if (!a.early || int(blockIdx.y) == experts_y) grid_wait();
   if (int(blockIdx.y) == experts_y) {
     for (int64_t s = rows_end(a) + threadIdx.x / CH; s < a.S; s += THREADS / CH) {
       const int64_t c = c0 + threadIdx.x % CH;
@@ -81,10 +82,13 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int b
     int before = 0;  // offsets[0 .. E - 1] at or before the row: the last of them begins its expert
     for (int64_t i = lane; i < a.E; i += 32) before += a.offsets[i] <= int64_t(blockIdx.y);
     e = __reduce_add_sync(~0u, before) - 1;
-    if (e < 0) return;
   }
-  segment(a, e, begin, end);
-  if (begin >= end || (by_row && begin != int64_t(blockIdx.y))) return;
+  begin = end = 0;
+  if (e >= 0) segment(a, e, begin, end);
+  if (begin >= end || (by_row && begin != int64_t(blockIdx.y))) {
+    grid_wait();  // a grid that ends has waited for the one before it, in every CTA
+    return;
+  }
 
   constexpr int64_t ES = KIND == S8 ? 1 : 2;
   const int64_t kbytes = a.K * ES, blocks = (kbytes + 63) / 64;
@@ -93,6 +97,19 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int b
   const bool oka = ca < I, okb = GLU ? ca < I : cb < I;
   const uint8_t* wa = a.W + e * a.stride_w + (oka ? ca : 0) * a.ldw + t * 16;
   const uint8_t* wb = a.W + e * a.stride_w + (okb ? cb : 0) * a.ldw + t * 16;
+
+  uint4 A[UNROLL], B[UNROLL];
+  auto load_weights = [&](int64_t b) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const bool in = (b + u) * 64 + t * 16 < kbytes;
+      A[u] = load16(wa + (b + u) * 64, in && oka);
+      B[u] = load16(wb + (b + u) * 64, in && okb);
+    }
+  };
+  load_weights(warp * UNROLL);  // in flight while the kernel before (the rows' producer) ends
+  if (a.early) grid_wait();
+  grid_release();
 
   for (int64_t r0 = begin; r0 < end; r0 += 8 * NT) {
     const uint8_t* xp[NT];
@@ -108,14 +125,8 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int b
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[n][i] = T(0);
+    if (r0 != begin) load_weights(warp * UNROLL);
     for (int64_t b = warp * UNROLL; b < blocks; b += WARPS * UNROLL) {
-      uint4 A[UNROLL], B[UNROLL];
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const bool in = (b + u) * 64 + t * 16 < kbytes;
-        A[u] = load16(wa + (b + u) * 64, in && oka);
-        B[u] = load16(wb + (b + u) * 64, in && okb);
-      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -127,6 +138,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int b
           mma<KIND>(acc[n], A[u].z, B[u].z, A[u].w, B[u].w, x.z, x.w);
         }
       }
+      if (b + WARPS * UNROLL < blocks) load_weights(b + WARPS * UNROLL);
     }
     __syncthreads();  // the sums of the previous rows have been read
 #pragma unroll
@@ -168,12 +180,10 @@ int launch_nt(const Args& a, cudaStream_t s) {
   const dim3 grid{unsigned(gx), unsigned(experts + (a.zero_behind && a.offsets ? 1 : 0))};
   const int64_t most = a.offsets ? (a.S + a.E - 1) / a.E * 2 : a.S;  // rows of a busy expert
   if (most <= 8)
-    rows_kernel<KIND, GLU, 1><<<grid, THREADS, 0, s>>>(a, by_row, int(experts));
-  else if (most <= 16)
-    rows_kernel<KIND, GLU, 2><<<grid, THREADS, 0, s>>>(a, by_row, int(experts));
-  else
-    rows_kernel<KIND, GLU, 4><<<grid, THREADS, 0, s>>>(a, by_row, int(experts));
-  return check_launch("rows_kernel");
+    return launch_dependent("rows_kernel", rows_kernel<KIND, GLU, 1>, grid, THREADS, 0, s, a, by_row, int(experts));
+  if (most <= 16)
+    return launch_dependent("rows_kernel", rows_kernel<KIND, GLU, 2>, grid, THREADS, 0, s, a, by_row, int(experts));
+  return launch_dependent("rows_kernel", rows_kernel<KIND, GLU, 4>, grid, THREADS, 0, s, a, by_row, int(experts));
 }
 
 }  // namespace

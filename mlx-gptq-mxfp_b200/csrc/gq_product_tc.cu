@@ -320,6 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                  "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
+  grid_wait();  // the barriers and TMEM above were set up while the kernel before ended
   if (warp == 2) {
     // Rows of every expert and the exclusive scan of their tiles. Offsets that run backwards
     // are raised to the largest before them, so that the tiles stay within S rows whatever
@@ -355,6 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   cluster_sync();
+  grid_release();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int tiles = ex.first_tile[E] * ct;  // below 2^31: checked by the host for any offsets
@@ -545,13 +547,14 @@ template <bool I8, bool GLU>
 int launch(const CUtensorMap& wmap, const XMaps& xmaps, const Args& a, Kind kind, unsigned grid, cudaStream_t s) {
   auto* k = tc_kernel<I8, GLU>;
   GQ_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_BYTES)));
-  k<<<grid, THREADS, SMEM_BYTES, s>>>(wmap, xmaps, a, kind);
-  return check_launch("tc_kernel");
+  return launch_dependent("tc_kernel", k, dim3(grid), THREADS, SMEM_BYTES, s, wmap, xmaps, a, kind);
 }
 
 // dst[s] = X[rows[s]] for the rows of every expert (a row of zeros where there is none).
 // HBM-bound copy: a warp per row, four 16-byte loads per lane in flight.
 __global__ void __launch_bounds__(256) gather_kernel(const Args a, uint4* __restrict__ dst, int64_t vecs) {
+  grid_wait();
+  grid_release();
   const int lane = threadIdx.x & 31;
   const int64_t last = rows_end(a), stride = int64_t(gridDim.x) * (blockDim.x >> 5);
   for (int64_t s = int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); s < last; s += stride) {
@@ -592,8 +595,8 @@ int launch_tc(const Args& a, Kind kind, bool glu, void* gathered, cudaStream_t s
   const int64_t row_bytes = a.K * int64_t(es);
   if (a.rows) {
     const int64_t warps = std::min<int64_t>(a.S, int64_t(sms) * 64);
-    gather_kernel<<<unsigned((warps + 7) / 8), 256, 0, s>>>(a, reinterpret_cast<uint4*>(gathered), row_bytes / 16);
-    st = check_launch("gather_kernel");
+    st = launch_dependent("gather_kernel", gather_kernel, dim3(unsigned((warps + 7) / 8)), 256, 0, s, a,
+                          reinterpret_cast<uint4*>(gathered), row_bytes / 16);
     if (st != GQ_OK) return st;
   }
   for (int b = 0; b < X_MAPS; ++b) {

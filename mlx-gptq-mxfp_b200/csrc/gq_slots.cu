@@ -43,6 +43,8 @@ template <typename I>
 __global__ void __launch_bounds__(THREADS)
     count_kernel(const I* __restrict__ index, int64_t T, int64_t k, int E, int64_t chunk, int32_t* __restrict__ counts) {
   __shared__ int32_t h[kMaxExperts + 1];
+  grid_wait();
+  grid_release();
   for (int e = threadIdx.x; e <= E; e += THREADS) h[e] = 0;
   __syncthreads();
   const int64_t i0 = int64_t(blockIdx.x) * chunk, i1 = i0 + chunk < T * k ? i0 + chunk : T * k;
@@ -61,6 +63,8 @@ __global__ void __launch_bounds__(THREADS)
   __shared__ int32_t next[kMaxExperts + 1];  // where the bin's next slot goes
   __shared__ int32_t total[kMaxExperts + 1], warp_sum[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bins = E + 1;
+  grid_wait();
+  grid_release();
   const int64_t slots = T * k, i0 = int64_t(blockIdx.x) * chunk, i1 = i0 + chunk < slots ? i0 + chunk : slots;
 
   // slots of every bin: all of them (total) and those of the chunks before this one (next)
@@ -142,6 +146,8 @@ __global__ void __launch_bounds__(256)
     combine_kernel(const T* __restrict__ y, int64_t S, int64_t ldy, const int32_t* __restrict__ slot,
                    const float* __restrict__ weights, int64_t tokens, int64_t k, int64_t N, T* __restrict__ out,
                    int64_t ldo) {
+  grid_wait();
+  grid_release();
   const int64_t per = N / V, i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= tokens * per) return;
   const int64_t t = i / per, c = (i % per) * V;
@@ -183,14 +189,14 @@ int route(const I* index, int64_t T, int64_t k, int64_t E, int32_t* tok, int32_t
           int32_t* counts, cudaStream_t s) {
   const int64_t chunk = chunk_size(T * k), n = chunks_of(T * k);
   if (n > 1) {
-    count_kernel<I><<<unsigned(n), THREADS, 0, s>>>(index, T, k, int(E), chunk, counts);
-    const int st = check_launch("count_kernel");
+    const int st = launch_dependent("count_kernel", count_kernel<I>, dim3(unsigned(n)), THREADS, 0, s, index, T, k,
+                                    int(E), chunk, counts);
     if (st != GQ_OK) return st;
   }
   const size_t smem = size_t(WARPS) * size_t(E + 1) * 2;  // up to 64 KB + 64
   GQ_CUDA_TRY(cudaFuncSetAttribute(place_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-  place_kernel<I><<<unsigned(n), THREADS, smem, s>>>(index, T, k, int(E), chunk, counts, tok, slot, offsets);
-  return check_launch("place_kernel");
+  return launch_dependent("place_kernel", place_kernel<I>, dim3(unsigned(n)), THREADS, smem, s, index, T, k, int(E),
+                          chunk, counts, tok, slot, offsets);
 }
 
 template <typename T>
@@ -199,11 +205,8 @@ int combine(const void* y, int64_t S, int64_t ldy, const int32_t* slot, const fl
   const bool wide = N % 8 == 0 && ldy % 8 == 0 && ldo % 8 == 0 && aligned16(y) && aligned16(out);
   const int64_t threads = tokens * (wide ? N / 8 : N);
   const unsigned grid = unsigned((threads + 255) / 256);
-  if (wide)
-    combine_kernel<T, 8><<<grid, 256, 0, s>>>((const T*)y, S, ldy, slot, weights, tokens, k, N, (T*)out, ldo);
-  else
-    combine_kernel<T, 1><<<grid, 256, 0, s>>>((const T*)y, S, ldy, slot, weights, tokens, k, N, (T*)out, ldo);
-  return check_launch("combine_kernel");
+  return launch_dependent("combine_kernel", wide ? combine_kernel<T, 8> : combine_kernel<T, 1>, dim3(grid), 256, 0, s,
+                          (const T*)y, S, ldy, slot, weights, tokens, k, N, (T*)out, ldo);
 }
 
 }  // namespace slots
