@@ -49,26 +49,38 @@ EncodeTiledFn tensor_map_encoder();
 // Launch that may begin while the kernel before it in the stream ends (programmatic
 // dependent launch): the kernel calls grid_wait() before it touches what earlier kernels
 // write, and grid_release() once it has (see there).
-template <typename... P, typename... A>
-int launch_dependent(const char* what, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
-                     A... args) {
+struct Cluster {
+  unsigned x, y;
+};
+
+template <typename... P>
+int launch_dependent_in(const char* what, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
+                        cudaStream_t s, Cluster cluster, P... args) {
   cudaLaunchConfig_t c = {};
   c.gridDim = grid;
   c.blockDim = dim3(threads);
   c.dynamicSmemBytes = smem;
   c.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster.x, at[1].val.clusterDim.y = cluster.y, at[1].val.clusterDim.z = 1;
   c.attrs = at;
-  c.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, P(args)...);
+  c.numAttrs = cluster.x ? 2 : 1;  // x = 0: as compiled
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();
     set_last_error("%s: %s", what, cudaGetErrorString(e));
     return GQ_ERR_CUDA;
   }
   return GQ_OK;
+}
+
+template <typename... P, typename... A>
+int launch_dependent(const char* what, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
+                     A... args) {
+  return launch_dependent_in<P...>(what, kernel, grid, threads, smem, s, Cluster{0, 0}, P(args)...);
 }
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -11,8 +11,7 @@ namespace {
 // kernel once per 128 .. 256: the first while a busy expert's rows fit one pass.
 bool by_rows(int64_t S, int64_t E, int engine) { return engine == 0 || (engine < 0 && S <= 8 * E); }
 
-int run(const char* what, const Args& a, Kind kind, bool glu, int engine, void* workspace, size_t workspace_bytes,
-        cudaStream_t s) {
+int check(const char* what, const Args& a, Kind kind, bool glu, int engine) {
   const int64_t es = kind == S8 ? 1 : 2;
   const int64_t I = glu ? a.N / 2 : a.N;
   GQ_REQUIRE(a.S >= 0 && a.S < (int64_t(1) << 31) && a.n_src >= 0 && a.n_src < (int64_t(1) << 31),
@@ -33,6 +32,14 @@ int run(const char* what, const Args& a, Kind kind, bool glu, int engine, void* 
   if (a.S == 0) return GQ_OK;
   GQ_REQUIRE(a.X && a.W && a.Y && a.n_src > 0, "%s: null pointer", what);
   GQ_REQUIRE(aligned16(a.X) && aligned16(a.W), "%s: X and W must be 16-byte aligned", what);
+  return GQ_OK;
+}
+
+int run(const char* what, const Args& a, Kind kind, bool glu, int engine, void* workspace, size_t workspace_bytes,
+        cudaStream_t s) {
+  const int st = check(what, a, kind, glu, engine);
+  if (st != GQ_OK || a.S == 0) return st;
+  const int64_t es = kind == S8 ? 1 : 2;
   if (by_rows(a.S, a.E, engine)) return launch_rows(a, kind, glu, s);
   const size_t need = a.rows ? size_t(a.S) * size_t(a.K * es) : 0;
   GQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
@@ -153,6 +160,22 @@ extern "C" int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, c
   GQ_REQUIRE(index && weights && out, "gq_expert_mlp: null pointer");
   GQ_REQUIRE(I % 8 == 0 && (!acts || ld_acts % 8 == 0), "gq_expert_mlp: activation rows must be 16-byte aligned");
   const MlpPlan p = mlp_plan(T, k, E, K, I, N, acts == nullptr);
+  if (prod::token_fits(T, k, E) && (acts || (workspace && workspace_bytes >= p.total && aligned16(workspace)))) {
+    prod::Args up = {}, dn = {};
+    if (!acts) acts = reinterpret_cast<uint8_t*>(workspace) + p.acts, ld_acts = I;
+    up.X = (const uint8_t*)X, up.n_src = T, up.ldx = 2 * ldx, up.E = E, up.S = 1, up.offsets = (const int64_t*)index;
+    up.W = (const uint8_t*)gate_up, up.N = 2 * I, up.K = K, up.ldw = 2 * ld_gate_up, up.stride_w = 2 * stride_gate_up;
+    up.Y = acts, up.ldy = ld_acts, up.out_dtype = dtype;
+    dn.X = (const uint8_t*)acts, dn.n_src = k, dn.ldx = 2 * ld_acts, dn.E = E, dn.S = 1, dn.offsets = up.offsets;
+    dn.W = (const uint8_t*)down, dn.N = N, dn.K = I, dn.ldw = 2 * ld_down, dn.stride_w = 2 * stride_down;
+    dn.Y = out, dn.ldy = N, dn.out_dtype = dtype;  // offsets: only checked for being there
+    GQ_REQUIRE(dtype == GQ_BF16 || dtype == GQ_F16, "gq_expert_mlp: rows and weights are bf16 or f16 (dtype %d)", dtype);
+    GQ_REQUIRE(index_bits == 32 || index_bits == 64, "gq_expert_mlp: indices have 32 or 64 bits, not %d", index_bits);
+    const prod::Kind kind = dtype == GQ_BF16 ? prod::BF16 : prod::F16;
+    int bad = prod::check("gq_expert_mlp", up, kind, true, -1);
+    if (bad == GQ_OK) bad = prod::check("gq_expert_mlp", dn, kind, false, -1);
+    return bad != GQ_OK ? bad : prod::launch_token(up, dn, kind, index, index_bits, k, weights, (cudaStream_t)stream);
+  }
   GQ_REQUIRE(workspace && workspace_bytes >= p.total && aligned16(workspace),
              "gq_expert_mlp: workspace too small (%zu < %zu)", workspace_bytes, p.total);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
@@ -185,6 +208,20 @@ extern "C" int gq_linear_int8(const void* X, int dtype, int64_t M, int64_t K, in
   GQ_REQUIRE(need && workspace && workspace_bytes >= need && aligned16(workspace),
              "gq_linear_int8: workspace too small (%zu < %zu)", workspace_bytes, need);
   const int64_t Kp = (K + 15) / 16 * 16;
+  if (X && Wq && ws && prod::linear_rows_fit(X, dtype, M, K, ldx)) {
+    prod::Args a = {};
+    a.X = (const uint8_t*)Wq, a.n_src = M, a.ldx = Kp, a.E = 1, a.S = M;  // X itself is not read as codes
+    a.W = (const uint8_t*)Wq, a.N = N, a.K = K, a.ldw = ldw, a.stride_w = N * ldw, a.ws = ws;
+    a.bias = bias, a.bias_dtype = bias_dtype, a.Y = Y, a.ldy = ldy, a.out_dtype = out_dtype;
+    GQ_REQUIRE(dtype == GQ_BF16 || dtype == GQ_F16 || dtype == GQ_F32, "gq_linear_int8: dtype %d", dtype);
+    GQ_REQUIRE(out_dtype == GQ_BF16 || out_dtype == GQ_F16 || out_dtype == GQ_F32, "gq_linear_int8: out dtype %d",
+               out_dtype);
+    GQ_REQUIRE(!bias || bias_dtype == GQ_BF16 || bias_dtype == GQ_F16 || bias_dtype == GQ_F32,
+               "gq_linear_int8: bias dtype %d", bias_dtype);
+    GQ_REQUIRE(ldx >= K, "gq_linear_int8: ldx < K");
+    const int st = prod::check("gq_linear_int8", a, prod::S8, false, -1);
+    return st != GQ_OK ? st : prod::launch_linear_rows(X, dtype, ldx, a, (cudaStream_t)stream);
+  }
   float* xs = reinterpret_cast<float*>(workspace);
   int8_t* q = reinterpret_cast<int8_t*>(workspace) + align256(size_t(M) * 4);
   const int st = gq_rtn_int8(X, dtype, M, K, ldx, q, Kp, Kp, xs, stream);

@@ -36,6 +36,14 @@ struct Args {
 };
 
 int launch_rows(const Args& a, Kind kind, bool glu, cudaStream_t s);
+// The expert MLP of one token (token_fits): up: X = the token, Y = acts (k rows); down: X =
+// acts, Y = the output row.
+bool token_fits(int64_t T, int64_t k, int64_t E);
+int launch_token(const Args& up, const Args& down, Kind kind, const void* index, int index_bits, int64_t k,
+                 const float* weights, cudaStream_t s);
+// One or two rows X (a.S) of dtype, quantized and multiplied in one launch.
+bool linear_rows_fit(const void* X, int dtype, int64_t M, int64_t K, int64_t ldx);
+int launch_linear_rows(const void* X, int dtype, int64_t ldx, const Args& a, cudaStream_t s);
 // gathered: with a row list, S * K elements, 16-byte aligned.
 int launch_tc(const Args& a, Kind kind, bool glu, void* gathered, cudaStream_t s);
 

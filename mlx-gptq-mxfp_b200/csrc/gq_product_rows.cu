@@ -186,7 +186,246 @@ int launch_nt(const Args& a, cudaStream_t s) {
   return launch_dependent("rows_kernel", rows_kernel<KIND, GLU, 4>, grid, THREADS, 0, s, a, by_row, int(experts));
 }
 
+// ---------------------------------------------------------------------------
+// One token. Its k slots are found in the index itself (no route launch) and summed inside
+// a cluster (no combine launch): two launches for the expert MLP of a decoding step, whose
+// time is that of reading k experts' weights and of what comes before the first load.
+// ---------------------------------------------------------------------------
+
+// 16 channels (glu: 8 gate, 8 up) times one row: v0 = channel c0 + threadIdx.x (up: v1), in
+// threads below CH. x: the row, in global memory, valid after wait().
+template <int KIND, bool GLU, typename Wait>
+__device__ __forceinline__ void one_row(const uint8_t* W, int64_t ldw, int64_t c0, int64_t I, int64_t kbytes,
+                                        const uint8_t* x, bool live, Wait wait, float& v0, float& v1) {
+  __shared__ float part[WARPS][2][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t ca = c0 + g, cb = GLU ? I + c0 + g : c0 + g + 8, blocks = (kbytes + 63) / 64;
+  const bool oka = live && ca < I, okb = live && (GLU ? ca < I : cb < I);
+  const uint8_t *wa = W + (oka ? ca : 0) * ldw + t * 16, *wb = W + (okb ? cb : 0) * ldw + t * 16;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t b = warp * UNROLL; b == warp * UNROLL || b < blocks; b += WARPS * UNROLL) {
+    uint4 A[UNROLL], B[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const bool in = (b + u) * 64 + t * 16 < kbytes;
+      A[u] = load16(wa + (b + u) * 64, in && oka);
+      B[u] = load16(wb + (b + u) * 64, in && okb);
+    }
+    if (b == warp * UNROLL) wait();
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      uint4 v = make_uint4(0, 0, 0, 0);  // column 0 of the mma is the row, the others are zeros
+      if (live && g == 0 && (b + u) * 64 + t * 16 < kbytes) v = *reinterpret_cast<const uint4*>(x + (b + u) * 64 + t * 16);
+      mma<KIND>(acc, A[u].x, B[u].x, A[u].y, B[u].y, v.x, v.y);
+      mma<KIND>(acc, A[u].z, B[u].z, A[u].w, B[u].w, v.z, v.w);
+    }
+  }
+  if (t == 0) part[warp][0][g] = acc[0], part[warp][1][g] = acc[2];  // column 0: channels g and g + 8
+  __syncthreads();
+  v0 = v1 = 0.0f;
+  if (threadIdx.x < (GLU ? 8 : 16)) {
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      v0 += part[w][GLU ? 0 : threadIdx.x >> 3][threadIdx.x & 7];
+      if (GLU) v1 += part[w][1][threadIdx.x & 7];
+    }
+  }
+}
+
+struct Token {
+  const void* index;  // [k] of index_bits
+  int index_bits, k, E;
+};
+
+// The expert of slot j (-1: dropped) and its place among the token's slots by (expert, position).
+__device__ __forceinline__ int token_slot(const Token& k, int j, int& place) {
+  const int lane = threadIdx.x & 31;
+  int64_t e = -1;
+  if (lane < k.k)
+    e = k.index_bits == 64 ? reinterpret_cast<const int64_t*>(k.index)[lane]
+                           : int64_t(reinterpret_cast<const int32_t*>(k.index)[lane]);
+  if (e < 0 || e >= k.E) e = -1;
+  const int mine = __shfl_sync(~0u, int(e), j);
+  place = __popc(__ballot_sync(~0u, e >= 0 && (e < mine || (e == mine && lane < j))));
+  return mine;
+}
+
+// acts[place] = silu(gate_e x) * (up_e x); blockIdx.y: the position. Y = acts.
+template <int KIND>
+__global__ void __launch_bounds__(THREADS) token_glu_kernel(const Args a, const Token k) {
+  grid_wait();
+  grid_release();
+  int place;
+  const int e = token_slot(k, blockIdx.y, place);
+  if (e < 0) return;
+  const int64_t I = a.N / 2, c0 = int64_t(blockIdx.x) * 8, ch = c0 + threadIdx.x;
+  float gate, up;
+  one_row<KIND, true>(a.W + e * a.stride_w, a.ldw, c0, I, a.K * 2, a.X, true, [] {}, gate, up);
+  if (threadIdx.x < 8 && ch < I) store_from_f32(a.Y, place * a.ldy + ch, swiglu(gate, up), a.out_dtype);
+}
+
+// out = sum over positions j, in order, of weights[j] * (down_e acts[place]): a cluster is
+// the k positions of one block of 16 channels. X = acts, Y = out.
+template <int KIND>
+__global__ void __launch_bounds__(THREADS) token_down_kernel(const Args a, const Token k, const float* weights) {
+  __shared__ float term[16];
+  int place;
+  const int e = token_slot(k, blockIdx.y, place);  // the index is older than the kernel before this one
+  const int64_t c0 = int64_t(blockIdx.x) * 16;
+  float v, unused;
+  one_row<KIND, false>(a.W + (e < 0 ? 0 : e) * a.stride_w, a.ldw, c0, a.N, a.K * 2, a.X + place * a.ldx, e >= 0,
+                       [] { grid_wait(); }, v, unused);
+  grid_release();
+  if (threadIdx.x < 16) term[threadIdx.x] = e < 0 ? 0.0f : weights[blockIdx.y] * v;
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (blockIdx.y == 0 && threadIdx.x < 16 && c0 + threadIdx.x < a.N) {
+    float sum = 0.0f;
+    for (int j = 0; j < k.k; ++j) {  // the cluster's rank is the position
+      uint32_t addr;
+      float y;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(&term[threadIdx.x])), "r"(j));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(addr) : "memory");
+      sum += y;
+    }
+    store_from_f32(a.Y, c0 + threadIdx.x, sum, a.out_dtype);
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int KIND>
+int launch_token_kind(const Args& up, const Args& down, const Token& k, const float* weights, cudaStream_t s) {
+  const int64_t I = up.N / 2;
+  const int st = launch_dependent("token_glu_kernel", token_glu_kernel<KIND>, dim3(unsigned((I + 7) / 8), unsigned(k.k)),
+                                  THREADS, 0, s, up, k);
+  if (st != GQ_OK) return st;
+  return launch_dependent_in<Args, Token, const float*>("token_down_kernel", token_down_kernel<KIND>,
+                                                        dim3(unsigned((down.N + 15) / 16), unsigned(k.k)), THREADS, 0,
+                                                        s, Cluster{1, unsigned(k.k)}, down, k, weights);
+}
+
+// ---------------------------------------------------------------------------
+// One or two rows through an 8-bit layer: every CTA quantizes the rows itself (they are a
+// few KB in L2, and the weights are on their way meanwhile) instead of waiting for a launch
+// that does. The codes are those of gq_rtn_int8: the same IEEE operations.
+// ---------------------------------------------------------------------------
+template <typename T, int M>
+__global__ void __launch_bounds__(THREADS)
+    linear_rows_kernel(const T* X, const int64_t ldx, const Args a) {
+  extern __shared__ __align__(16) int8_t codes[];  // [M][K]
+  __shared__ uint32_t max_bits[M][WARPS];
+  __shared__ int32_t part[WARPS][4][32];
+  grid_wait();
+  grid_release();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t c0 = int64_t(blockIdx.x) * 16, ca = c0 + g, cb = ca + 8, blocks = (a.K + 63) / 64;
+  const bool oka = ca < a.N, okb = cb < a.N;
+  const uint8_t *wa = a.W + (oka ? ca : 0) * a.ldw + t * 16, *wb = a.W + (okb ? cb : 0) * a.ldw + t * 16;
+  uint4 A[UNROLL], B[UNROLL];
+  auto load_weights = [&](int64_t b) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const bool in = (b + u) * 64 + t * 16 < a.K;
+      A[u] = load16(wa + (b + u) * 64, in && oka);
+      B[u] = load16(wb + (b + u) * 64, in && okb);
+    }
+  };
+  load_weights(warp * UNROLL);
+  constexpr int V = 16 / int(sizeof(T));  // elements per load
+  float scale[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    uint32_t bits = 0;
+    for (int64_t c = threadIdx.x * V; c < a.K; c += THREADS * V) {
+      T v[V];
+      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(X + m * ldx + c);
+#pragma unroll
+      for (int i = 0; i < V; ++i) bits = max(bits, __float_as_uint(to_f32<T>(v[i])) & 0x7FFFFFFFu);
+    }
+    bits = __reduce_max_sync(~0u, bits);
+    if (lane == 0) max_bits[m][warp] = bits;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) bits = max(bits, max_bits[m][w]);
+    scale[m] = __uint_as_float(bits) / 127.0f;
+    for (int64_t c = threadIdx.x * V; c < a.K; c += THREADS * V) {
+      T v[V];
+      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(X + m * ldx + c);
+      uint32_t word[V / 4];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int q = scale[m] > 0.0f ? max(-127, min(127, __float2int_rn(to_f32<T>(v[i]) / scale[m]))) : 0;
+        word[i / 4] = (i & 3 ? word[i / 4] : 0u) | (uint32_t(q) & 0xFFu) << (8 * (i & 3));
+      }
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) reinterpret_cast<uint32_t*>(codes + m * a.K + c)[i] = word[i];
+    }
+  }
+  __syncthreads();
+  int32_t acc[4] = {0, 0, 0, 0};
+  for (int64_t b = warp * UNROLL; b < blocks; b += WARPS * UNROLL) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (g < M && (b + u) * 64 + t * 16 < a.K)
+        x = *reinterpret_cast<const uint4*>(codes + g * a.K + (b + u) * 64 + t * 16);
+      mma<S8>(acc, A[u].x, B[u].x, A[u].y, B[u].y, x.x, x.y);
+      mma<S8>(acc, A[u].z, B[u].z, A[u].w, B[u].w, x.z, x.w);
+    }
+    if (b + WARPS * UNROLL < blocks) load_weights(b + WARPS * UNROLL);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[warp][i][lane] = acc[i];
+  __syncthreads();
+  // accumulator i of lane (g, t): channel g + 8 (i / 2), row 2 t + i % 2
+  if (threadIdx.x < 16 * M) {
+    const int c = threadIdx.x & 15, m = threadIdx.x >> 4;
+    const int64_t ch = c0 + c;
+    if (ch < a.N) {
+      int32_t sum = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) sum += part[w][(c >> 3) * 2 + m][(c & 7) * 4];
+      float y = float(sum) * (m == 0 ? scale[0] : scale[M - 1]) * a.ws[ch];
+      if (a.bias) y = y + load_as_f32(a.bias, ch, a.bias_dtype);
+      store_from_f32(a.Y, m * a.ldy + ch, y, a.out_dtype);
+    }
+  }
+}
+
+template <typename T>
+int linear_rows(const void* X, int64_t ldx, const Args& a, cudaStream_t s) {
+  const dim3 grid(unsigned((a.N + 15) / 16));
+  const size_t smem = size_t(a.S) * size_t(a.K);
+  return launch_dependent("linear_rows_kernel", a.S == 1 ? linear_rows_kernel<T, 1> : linear_rows_kernel<T, 2>, grid,
+                          THREADS, smem, s, reinterpret_cast<const T*>(X), ldx, a);
+}
+
 }  // namespace
+
+bool token_fits(int64_t T, int64_t k, int64_t E) { return T == 1 && k <= 8 && E < (int64_t(1) << 31); }
+
+int launch_token(const Args& up, const Args& down, Kind kind, const void* index, int index_bits, int64_t k,
+                 const float* weights, cudaStream_t s) {
+  const Token t = {index, index_bits, int(k), int(up.E)};
+  return kind == F16 ? launch_token_kind<F16>(up, down, t, weights, s)
+                     : launch_token_kind<BF16>(up, down, t, weights, s);
+}
+
+bool linear_rows_fit(const void* X, int dtype, int64_t M, int64_t K, int64_t ldx) {
+  const int64_t es = dtype == GQ_F32 ? 4 : 2;
+  return M <= 2 && K % 16 == 0 && M * K <= 32768 && aligned16(X) && (M == 1 || ldx * es % 16 == 0);
+}
+
+int launch_linear_rows(const void* X, int dtype, int64_t ldx, const Args& a, cudaStream_t s) {
+  if (dtype == GQ_BF16) return linear_rows<__nv_bfloat16>(X, ldx, a, s);
+  if (dtype == GQ_F16) return linear_rows<__half>(X, ldx, a, s);
+  return linear_rows<float>(X, ldx, a, s);
+}
 
 int launch_rows(const Args& a, Kind kind, bool glu, cudaStream_t s) {
   if (kind == S8) return glu ? launch_nt<S8, true>(a, s) : launch_nt<S8, false>(a, s);

@@ -251,6 +251,43 @@ def test_expert_mlp(dtype, T, E, k, C, I):
     assert torch.equal(out, expert_mlp(x, idx.int(), wt, gate_up, down))  # without acts, 32-bit indices
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["i32", "i64"])
+@pytest.mark.parametrize("picks,E,C,I,N", [
+    ([3], 8, 64, 32, 64), ([7, 0, 5, 2], 8, 2048, 768, 2048), ([4, 9, 4, -1, 0, 12, 4, 11], 12, 200, 40, 136),
+    ([1, 1], 2, 72, 8, 24), ([-1, 5, 6], 5, 64, 32, 64), (list(range(9, 0, -1)), 10, 128, 64, 96)])
+def test_expert_mlp_of_one_token(dtype, index, picks, E, C, I, N):
+    """One token has its own form for up to eight positions: dropped positions, the same expert twice,
+    and nine positions, which take the general form. The sum's terms are float32 or rounded to
+    the inputs' type: the tolerance counts the rounding."""
+    from mlx_gptq_b200 import expert_mlp
+
+    g = _gen(len(picks) * C + I)
+    x = _randn(g, 1, C).to(dtype)
+    gate_up, down = (_randn(g, E, 2 * I, C) * 0.05).to(dtype), (_randn(g, E, N, I) * 0.2).to(dtype)
+    idx = torch.tensor([picks], device="cuda").to(index)
+    k = len(picks)
+    wt = torch.rand(1, k, generator=g, device="cuda")
+    acts = torch.full((k, I), 5.0, dtype=dtype, device="cuda")
+    out = expert_mlp(x, idx, wt, gate_up, down, acts=acts)
+    order = sorted((e, j) for j, e in enumerate(picks) if 0 <= e < E)
+    n = len(order)
+    counts = [sum(1 for e, _ in order if e == i) for i in range(E)]
+    zeros = torch.zeros(n, dtype=torch.int64, device="cuda")
+    h, herr = _reference(x.double(), gate_up.double(), counts, zeros, True, n)
+    _assert_close(acts[:n], h, herr, "acts")
+    assert bool((acts[n:] == 5).all())
+    y, yerr = _reference(acts[:n].double(), down.double(), counts, torch.arange(n, device="cuda"), False, n)
+    w = torch.stack([wt[0, j] for _, j in order]).double()[:, None] if n else wt[0, :0, None].double()
+    u = torch.finfo(dtype).eps / 2
+    err = ((yerr + u * (y.abs() + yerr) + 2.0 ** -25 + (k + 1) * 2.0 ** -24 * y.abs()) * w).sum(0)
+    _assert_close(out[0], (y * w).sum(0), err, "out")
+    assert torch.equal(out, expert_mlp(x, idx, wt, gate_up, down))
+    wide = torch.full((1, N + 9), 3.0, dtype=dtype, device="cuda")
+    assert torch.equal(out, expert_mlp(x, idx, wt, gate_up, down, out=wide[:, 4:4 + N]))
+    assert bool((wide[:, :4] == 3).all()) and bool((wide[:, 4 + N:] == 3).all())
+
+
 def _codes(x):
     """The grid in torch, operation by operation."""
     x = x.float()
@@ -402,20 +439,27 @@ def test_expert_mlp_in_8_bits():
     _assert_close(out, want, err)
 
 
-@pytest.mark.parametrize("M,K,N", [(1, 4096, 512), (70, 100, 33), (400, 1024, 300)])
-def test_linear_int8(M, K, N):
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("B,M,K,N", [(1, 1, 4096, 512), (2, 1, 4096, 515), (1, 1, 20, 33), (1, 1, 32768, 40),
+                                     (1, 2, 20480, 40), (2, 70, 100, 33), (2, 400, 1024, 300)])
+def test_linear_int8(dtype, B, M, K, N):
     from mlx_gptq_b200 import linear_int8, rtn_quantize_int8
 
     g = _gen(M + N)
-    x = _randn(g, 2, M, K).to(BF16)
+    x = _randn(g, B, M, K).to(dtype)
+    if B * M > 1:
+        x[0, 0] = 0
     wq, ws = rtn_quantize_int8(_randn(g, N, K) * 0.05)
     bias = _randn(g, N).to(BF16)
     y = linear_int8(x, wq, ws, bias)
     q, s = _codes(x.reshape(-1, K))
     want, err = _int8_reference(q, s, wq, ws, bias)
-    assert y.shape == (2, M, N) and y.dtype == BF16
+    assert y.shape == (B, M, N) and y.dtype == dtype
     _assert_close(y.reshape(-1, N), want, err)
-    assert linear_int8(x[:, :0], wq, ws).shape == (2, 0, N)
+    wide = torch.zeros(B, M, K + 16, dtype=dtype, device="cuda")  # rows of a wider tensor
+    wide[..., 16:] = x
+    assert torch.equal(y, linear_int8(wide[..., 16:], wq, ws, bias))
+    assert linear_int8(x[:, :0], wq, ws).shape == (B, 0, N)
 
 
 @pytest.mark.parametrize("T", [1, 700], ids=["token", "batch"])
