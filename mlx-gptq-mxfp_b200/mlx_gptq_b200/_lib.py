@@ -6,6 +6,7 @@ present, calls raise instead of falling back to anything else.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -120,7 +121,17 @@ def check(status: int, what: str) -> None:
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The device's current stream (default: the current device's) as a pointer."""
+    idx = None if device is None else device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """A context in which launches go to `device`, whatever device is current."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

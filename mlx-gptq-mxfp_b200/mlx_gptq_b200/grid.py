@@ -9,8 +9,6 @@ tensors.
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib as L
@@ -114,16 +112,15 @@ def _int8_codes(rows: torch.Tensor, columns: int) -> tuple[torch.Tensor, torch.T
     n, C = rows.shape
     if (C > 1 and rows.stride(1) != 1) or (n > 1 and rows.stride(0) < C):
         rows = rows.contiguous()
-    dev = rows.device
+    dev, code = rows.device, _dtype_code(rows.dtype)
     q = torch.empty(n, columns, dtype=torch.int8, device=dev)
     s = torch.empty(n, dtype=torch.float32, device=dev)
-    with contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
-        L.check(L.lib().gq_rtn_int8(L.ptr(rows), _dtype_code(rows.dtype), n, C, rows.stride(0) if n > 1 else C,
+    with L.on(dev):
+        L.check(L.lib().gq_rtn_int8(L.ptr(rows), code, n, C, rows.stride(0) if n > 1 else C,
                                     L.ptr(q), columns, columns, L.ptr(s), L.stream_ptr(dev)), "rtn_quantize_int8")
     return q, s
 
 
-@torch.no_grad()
 def rtn_quantize_int8(W: torch.Tensor):
     """RTN in 8-bit integers, symmetric, one scale per row (no reference counterpart): the
     grid of products.matmul_int8, for weights (a row is an output channel) and for
@@ -135,7 +132,9 @@ def rtn_quantize_int8(W: torch.Tensor):
     L.require_cuda(W)
     if W.dim() == 0 or W.shape[-1] == 0:
         raise ValueError("rtn_quantize_int8 needs rows of at least one column")
-    _dtype_code(W.dtype)
+    W = W.detach()
+    if W.dim() == 2:
+        return _int8_codes(W, W.shape[1])
     q, s = _int8_codes(W.reshape(-1, W.shape[-1]), W.shape[-1])
     return q.reshape(W.shape), s.reshape(W.shape[:-1])
 

@@ -20,7 +20,6 @@ They have no backward: with gradients enabled, inputs that require them are refu
 
 from __future__ import annotations
 
-import contextlib
 import functools
 
 import torch
@@ -41,16 +40,7 @@ def _forward_only(what: str, *tensors) -> torch.device:
     return dev
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(dev: torch.device):
-    """Launches go to `dev`, whatever device is current."""
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-
-def _stream(dev: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+_on, _stream = L.on, L.stream_ptr
 
 
 def _status(dev: torch.device) -> int:
@@ -85,6 +75,8 @@ def _operand(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     padded with zeros to a multiple of 16 bytes."""
     m = 16 // t.element_size()
     K = t.shape[-1]
+    if t.is_contiguous() and K % m == 0 and t.data_ptr() % 16 == 0:
+        return t, K, t.shape[-2] * K
 
     def strides(x):
         ld = x.stride(-2) if x.shape[-2] > 1 else x.shape[-1]
@@ -118,11 +110,20 @@ def _offsets(offsets: torch.Tensor, E: int, dev: torch.device) -> torch.Tensor:
 def _output(out, shape, dtype, dev, name="out") -> torch.Tensor:
     if out is None:
         return torch.empty(shape, dtype=dtype, device=dev)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != dev:
+    if out.shape != shape or out.dtype != dtype or out.device != dev:
         raise ValueError(f"{name} must be {dtype} {list(shape)} on {dev}")
-    if (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1]):
+    if not out.is_contiguous() and ((shape[1] > 1 and out.stride(1) != 1) or
+                                    (shape[0] > 1 and out.stride(0) < shape[1])):
         raise ValueError(f"{name} must have whole rows that do not overlap")
     return out
+
+
+_INDEX_BITS = {torch.int32: 32, torch.int64: 64}
+
+
+def _weights(w: torch.Tensor) -> torch.Tensor:
+    """Routing weights as the kernels read them: float32, contiguous."""
+    return w if w.dtype == torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -160,7 +161,7 @@ def route_slots(top_k_index: torch.Tensor, num_experts: int) -> tuple[torch.Tens
     behind the last); slot int32 [T, k], where each went (-1 if dropped); offsets int64
     [num_experts + 1], the first slot of every expert."""
     dev = L.require_cuda(top_k_index)
-    if top_k_index.dim() != 2 or top_k_index.dtype not in (torch.int32, torch.int64) or top_k_index.shape[1] == 0:
+    if top_k_index.dim() != 2 or top_k_index.dtype not in _INDEX_BITS or top_k_index.shape[1] == 0:
         raise ValueError("top_k_index must be int32 or int64 [tokens, k]")
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"{num_experts} experts, 1 to {MAX_EXPERTS}")
@@ -172,7 +173,7 @@ def route_slots(top_k_index: torch.Tensor, num_experts: int) -> tuple[torch.Tens
     ws_bytes = _size("gq_route_slots_workspace_size", T, k, num_experts)
     ws = _scratch(ws_bytes, dev)
     with _on(dev):
-        L.check(L.lib().gq_route_slots(L.ptr(idx), 8 * idx.element_size(), T, k, num_experts, L.ptr(tok), L.ptr(slot),
+        L.check(L.lib().gq_route_slots(L.ptr(idx), _INDEX_BITS[idx.dtype], T, k, num_experts, L.ptr(tok), L.ptr(slot),
                                        L.ptr(offsets), L.ptr(ws), ws_bytes, _stream(dev)), "route_slots")
     return tok, slot, offsets
 
@@ -195,7 +196,7 @@ def combine_slots(y: torch.Tensor, slot: torch.Tensor, weights: torch.Tensor,
     out = _output(out, (T, N), y.dtype, dev)
     if T == 0 or N == 0:
         return out
-    sl, w = slot.contiguous(), weights.to(torch.float32).contiguous()
+    sl, w = slot.contiguous(), _weights(weights)
     with _on(dev):
         L.check(L.lib().gq_combine_slots(L.ptr(y), L.DTYPE_CODE[y.dtype], S, _ld(y), L.ptr(sl), L.ptr(w), T, k, N,
                                          L.ptr(out), _ld(out), _stream(dev)), "combine_slots")
@@ -251,26 +252,26 @@ def expert_mlp(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.
     are left alone). Returns [T, C']."""
     dev = _forward_only("expert_mlp", x, top_k_index, top_k_weights, gate_up, down, acts, out)
     _check_pair(x, gate_up, 3)
-    if down.dim() != 3 or down.shape[0] != gate_up.shape[0] or 2 * down.shape[2] != gate_up.shape[1]:
-        raise ValueError(f"shapes: gate_up [E, 2 I, C] {list(gate_up.shape)}, down [E, C', I] {list(down.shape)}")
-    if top_k_index.dim() != 2 or top_k_index.shape[0] != x.shape[0] or top_k_weights.shape != top_k_index.shape:
+    dtype, shape_up, shape_down, shape_idx = x.dtype, gate_up.shape, down.shape, top_k_index.shape
+    if len(shape_down) != 3 or shape_down[0] != shape_up[0] or 2 * shape_down[2] != shape_up[1] or 0 in shape_down:
+        raise ValueError(f"shapes: gate_up [E, 2 I, C] {list(shape_up)}, down [E, C', I] {list(shape_down)}")
+    if len(shape_idx) != 2 or shape_idx[0] != x.shape[0] or top_k_weights.shape != shape_idx or shape_idx[1] == 0:
         raise ValueError("top_k_index and top_k_weights must be [tokens, k]")
-    T, k = top_k_index.shape
-    I = down.shape[2]
     if not top_k_weights.is_floating_point():
         raise ValueError("top_k_weights must be floating point")
-    if top_k_index.dtype not in (torch.int32, torch.int64) or k == 0:
+    if top_k_index.dtype not in _INDEX_BITS:
         raise ValueError("top_k_index must be int32 or int64 [tokens, k]")
-    for w in (gate_up, down):
-        if x.dtype != w.dtype or x.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"rows and weights must all be bf16 or f16, not {x.dtype} and {w.dtype}")
-    E, N = down.shape[:2]
+    if dtype not in (torch.bfloat16, torch.float16) or gate_up.dtype != dtype or down.dtype != dtype:
+        raise ValueError(f"rows and weights must all be bf16 or f16, not {dtype}, {gate_up.dtype} and {down.dtype}")
+    (T, k), (E, N, I) = shape_idx, shape_down
+    ld_acts = 0
     if acts is not None:
-        acts = _output(acts, (T * k, I), x.dtype, dev, "acts")
-    out = _output(out, (T, N), x.dtype, dev)
+        acts = _output(acts, (T * k, I), dtype, dev, "acts")
+        ld_acts = _ld(acts)
+    out = _output(out, (T, N), dtype, dev)
     if T == 0:
         return out
-    if I % 8 or (acts is not None and (_ld(acts) % 8 or acts.data_ptr() % 16)):
+    if I % 8 or (acts is not None and (ld_acts % 8 or acts.data_ptr() % 16)):
         # activation rows that the second product cannot read in place
         tok, slot, offsets = route_slots(top_k_index, E)
         h = matmul_grouped(x, gate_up, offsets, rows=tok, glu=True, out=acts)
@@ -279,16 +280,15 @@ def expert_mlp(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.
     xo, ldx, _ = _operand(x)
     gu, ld_gu, stride_gu = _operand(gate_up)
     dn, ld_dn, stride_dn = _operand(down)
-    idx, wt = top_k_index.contiguous(), top_k_weights.to(torch.float32).contiguous()
+    idx, wt = top_k_index.contiguous(), _weights(top_k_weights)
     K = gu.shape[2]
     nbytes = _size("gq_expert_mlp_workspace_size", T, k, E, K, I, N, int(acts is None))
     ws = _scratch(nbytes, dev)
     with _on(dev):
         L.check(L.lib().gq_expert_mlp(
-            xo.data_ptr(), L.DTYPE_CODE[x.dtype], T, ldx, idx.data_ptr(), 8 * idx.element_size(), wt.data_ptr(), k,
-            gu.data_ptr(), ld_gu, stride_gu, dn.data_ptr(), ld_dn, stride_dn, E, K, I, N, L.ptr(acts),
-            0 if acts is None else _ld(acts), out.data_ptr(), _ld(out), ws.data_ptr(), nbytes, _status(dev),
-            _stream(dev)), "expert_mlp")
+            xo.data_ptr(), L.DTYPE_CODE[dtype], T, ldx, idx.data_ptr(), _INDEX_BITS[idx.dtype], wt.data_ptr(), k,
+            gu.data_ptr(), ld_gu, stride_gu, dn.data_ptr(), ld_dn, stride_dn, E, K, I, N, L.ptr(acts), ld_acts,
+            out.data_ptr(), _ld(out), L.ptr(ws), nbytes, _status(dev), _stream(dev)), "expert_mlp")
     return out
 
 
