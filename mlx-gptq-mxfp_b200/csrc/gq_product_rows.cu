@@ -61,7 +61,7 @@ __device__ __forceinline__ void mma(T (&c)[4], uint32_t a0, uint32_t a1, uint32_
 // behind. The weights wait for the expert, so it is found in one step of memory latency:
 // every lane of a warp counts the offsets at or before the row.
 template <int KIND, bool GLU, int NT>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const Args a, const int by_row, const int experts_y) {
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : (NT == 2 ? 3 : 2)) rows_kernel(const Args a, const int by_row, const int experts_y) {
   typedef typename Acc<KIND>::T T;
   __shared__ T part[WARPS][NT][4][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;

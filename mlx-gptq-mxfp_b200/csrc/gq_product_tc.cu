@@ -48,14 +48,20 @@ constexpr uint32_t A_BYTES = 128 * 128;  // 128 channels x 128 bytes of k
 constexpr int X_MAPS = 4;                // TMA boxes of X: 128, 64, 32 and 16 rows
 constexpr uint32_t kEvenCta = 0xFEFFFFFFu;  // shared::cluster address -> even CTA of the pair
 
-constexpr int NMAX = 256;  // rows per tile
-constexpr uint32_t B_BYTES = uint32_t(NMAX / 2) * 128;
-constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int STAGES = 6;
-constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ +
-                              12 * (kMaxExperts + 1) /*tiles and rows of every expert*/;
-
-static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+// Two tile widths. 256 rows for throughput. 64 rows where experts have few (decoding
+// batches): the time is then that of streaming the weights, a tile's loads are nearly all
+// weights, and 10 stages of 20 KB keep 160 KB of them in flight per SM where 6 of 32 KB
+// keep 96.
+template <int NMAX>
+struct Shape {
+  static constexpr uint32_t B_BYTES = uint32_t(NMAX / 2) * 128;
+  static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = NMAX == 256 ? 6 : 10;
+  static constexpr size_t SMEM_BYTES = size_t(STAGES) * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/ +
+                                       12 * (kMaxExperts + 1) /*tiles and rows of every expert*/;
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+  static_assert((2 * STAGES + 4) * 8 + 8 <= 256, "barriers");
+};
 
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -143,8 +149,8 @@ __device__ __forceinline__ uint32_t instruction_desc(Kind kind, int n) {
 struct Ring {
   int stage = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void step() {
-    if (++stage == STAGES) stage = 0, phase ^= 1;
+  __device__ __forceinline__ void step(int stages) {
+    if (++stage == stages) stage = 0, phase ^= 1;
   }
 };
 
@@ -165,7 +171,7 @@ struct Experts {
 };
 
 // Tile q of the list: expert by expert, row tile by row tile, its channel blocks.
-__device__ __forceinline__ Tile tile_of(int q, const Experts& x, int E, int ct, int step) {
+__device__ __forceinline__ Tile tile_of(int q, const Experts& x, int E, int ct, int step, int most) {
   int lo = 0, hi = E;  // last expert whose tiles begin at or before q / ct
   const int r = q / ct;
   while (hi - lo > 1) {
@@ -173,8 +179,8 @@ __device__ __forceinline__ Tile tile_of(int q, const Experts& x, int E, int ct, 
     if (x.first_tile[mid] <= r) lo = mid; else hi = mid;
   }
   const int n = x.end[lo] - x.begin[lo];
-  const int tiles = (n + NMAX - 1) / NMAX;
-  const int per = ((n + tiles - 1) / tiles + step - 1) / step * step;  // <= NMAX, a multiple of step
+  const int tiles = (n + most - 1) / most;
+  const int per = ((n + tiles - 1) / tiles + step - 1) / step * step;  // <= most, a multiple of step
   Tile t;
   t.expert = lo;
   t.block = q - r * ct;
@@ -276,11 +282,12 @@ __device__ __forceinline__ void store_any_block(const Args& a, int64_t row0, int
   }
 }
 
-template <bool I8, bool GLU>
+template <bool I8, bool GLU, int NMAX>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ XMaps xmaps, const Args a,
-              const Kind kind) {
-  constexpr int STEP = I8 ? 32 : 16;
+              const Kind kind, const int most) {  // most: rows per tile, a multiple of 32 up to NMAX
+  constexpr int STEP = I8 ? 32 : 16, STAGES = Shape<NMAX>::STAGES, BLOCKS = NMAX / 64;
+  constexpr uint32_t STAGE_BYTES = Shape<NMAX>::STAGE_BYTES;
   constexpr int KSTEP = I8 ? 128 : 64;  // elements per stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -340,7 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       int32_t start = __shfl_up_sync(~0u, stop, 1);
       start = max(int32_t(begin), lane ? start : reached);
       if (start > stop) start = stop;
-      const int32_t mine = (stop - start + NMAX - 1) / NMAX;
+      const int32_t mine = (stop - start + most - 1) / most;
       int32_t incl = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -372,10 +379,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     int n_chunk = 0;
     bool ok = true;
     for (int q = pair; q < tiles && ok; q += pairs) {
-      const Tile t = tile_of(q, ex, E, ct, STEP);
-      Sum acc[4][32];
+      const Tile t = tile_of(q, ex, E, ct, STEP, most);
+      Sum acc[BLOCKS][32];
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
         for (int j = 0; j < 32; ++j) acc[b][j] = Sum(0);
       for (int k0 = 0; k0 < KT; k0 += chunk, ++n_chunk) {
@@ -386,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         tc_fence_after();
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < BLOCKS; ++b) {
           const int c = part * 32 + 64 * b;
           if (c < t.rows) {
             uint32_t r[32];
@@ -413,7 +420,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         if (a.bias) bias = load_as_f32(a.bias, ch, a.bias_dtype);
       }
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < BLOCKS; ++b) {
         const int c = part * 32 + 64 * b;
         if (c < t.rows) {
           float xs_lane = 0.0f;
@@ -448,7 +455,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       Ring ring;
       bool ok = true, lapped = false;
       for (int q = pair; q < tiles && ok; q += pairs) {
-        const Tile t = tile_of(q, ex, E, ct, STEP);
+        const Tile t = tile_of(q, ex, E, ct, STEP, most);
         const int half = t.n / 2, x_rows = (half + 15) / 16 * 16;  // <= 128
         const uint32_t bytes = A_BYTES + uint32_t(x_rows) * 128;
         const int ch = (t.block * 2 + int(rank)) * (GLU ? 64 : 128), y = int(t.row0) + int(rank) * half;
@@ -467,7 +474,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               tma_2d(st + A_BYTES + r * 128, &xmaps.box[b], kt * KSTEP, y + r, &full[s]);
               r += 128 >> b;
             }
-          ring.step();
+          ring.step(STAGES);
           lapped |= ring.stage == 0;
         }
       }
@@ -483,7 +490,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       bool ok = true;
       const uint64_t desc = umma_desc_sw128(smem_u32(smem), 16, 1024);  // + (byte offset >> 4)
       for (int q = pair; q < tiles && ok; q += pairs) {
-        const Tile t = tile_of(q, ex, E, ct, STEP);
+        const Tile t = tile_of(q, ex, E, ct, STEP, most);
         const uint32_t idesc = instruction_desc(kind, t.n);
         for (int k0 = 0; k0 < KT && ok; k0 += chunk, ++n_chunk) {
           const int buf = n_chunk & 1, k1 = k0 + chunk < KT ? k0 + chunk : KT;
@@ -506,7 +513,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               mma<I8>(d, ad + 2 * kk, bd + 2 * kk, idesc, more);
             }
             commit(&empty[s]);  // frees the stage once these MMAs have read it
-            ring.step();
+            ring.step(STAGES);
           }
           if (ok) commit(&tfull[buf]);
         }
@@ -543,11 +550,15 @@ int encode(CUtensorMap* map, const void* base, Kind kind, int rank, const cuuint
   return GQ_OK;
 }
 
-template <bool I8, bool GLU>
-int launch(const CUtensorMap& wmap, const XMaps& xmaps, const Args& a, Kind kind, unsigned grid, cudaStream_t s) {
-  auto* k = tc_kernel<I8, GLU>;
-  GQ_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(SMEM_BYTES)));
-  return launch_dependent("tc_kernel", k, dim3(grid), THREADS, SMEM_BYTES, s, wmap, xmaps, a, kind);
+template <int NMAX>
+int launch(const CUtensorMap& wmap, const XMaps& xmaps, const Args& a, Kind kind, bool glu, int most, unsigned grid,
+           cudaStream_t s) {
+  const bool i8 = kind == S8;
+  auto* k = i8 ? (glu ? tc_kernel<true, true, NMAX> : tc_kernel<true, false, NMAX>)
+               : (glu ? tc_kernel<false, true, NMAX> : tc_kernel<false, false, NMAX>);
+  constexpr size_t smem = Shape<NMAX>::SMEM_BYTES;
+  GQ_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  return launch_dependent("tc_kernel", k, dim3(grid), THREADS, smem, s, wmap, xmaps, a, kind, most);
 }
 
 // dst[s] = X[rows[s]] for the rows of every expert (a row of zeros where there is none).
@@ -572,6 +583,24 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, uint4* __rest
         if (v0 + 32 * i < vecs) dst[s * vecs + v0 + 32 * i] = r[i];
     }
   }
+}
+
+// Rows per tile. Grouped: 256, the counts are on the device. Dense: the number of row tiles
+// whose last round of tiles over the CTA pairs is filled best; a k-step of a tile of n rows
+// takes the loads of 128 channels and n / 2 rows (128 bytes each, 47 bytes per cycle), so
+// a round costs 16384 + 64 n. 1357 rows x 4096 channels: 96 tiles of 240 rows on 74
+// pairs are two rounds, 144 tiles of 160 rows are two shorter ones.
+int rows_per_tile(const Args& a, int64_t pairs, int64_t blocks) {
+  if (a.offsets) return 256;
+  int best = 256;
+  double best_time = 1e300;
+  for (int rows = 256; rows >= 64; rows -= 32) {
+    const int64_t tiles = (a.S + rows - 1) / rows, n = ((a.S + tiles - 1) / tiles + 31) / 32 * 32;
+    const int64_t rounds = (tiles * blocks + pairs - 1) / pairs;
+    const double time = double(rounds) * (16384.0 + 64.0 * double(n));
+    if (time < best_time) best_time = time, best = rows;
+  }
+  return best;
 }
 
 }  // namespace
@@ -606,13 +635,14 @@ int launch_tc(const Args& a, Kind kind, bool glu, void* gathered, cudaStream_t s
     st = encode(&xmaps.box[b], a.rows ? gathered : (const void*)a.X, kind, 2, xdims, xstrides, xbox);
     if (st != GQ_OK) return st;
   }
-  const int64_t blocks = (a.N + 255) / 256;
-  const int64_t most = blocks * (a.S / NMAX + std::min(a.S, a.E));  // at least the number of tiles
-  GQ_REQUIRE(most < (int64_t(1) << 31) - 65536, "product: too many tiles");
-  const unsigned grid = unsigned(2 * std::min<int64_t>(std::max(sms / 2, 1), std::max<int64_t>(most, 1)));
-  if (kind == S8)
-    return glu ? launch<true, true>(wmap, xmaps, a, kind, grid, s) : launch<true, false>(wmap, xmaps, a, kind, grid, s);
-  return glu ? launch<false, true>(wmap, xmaps, a, kind, grid, s) : launch<false, false>(wmap, xmaps, a, kind, grid, s);
+  const int64_t pairs = std::max(sms / 2, 1), blocks = (a.N + 255) / 256;
+  const bool narrow = a.S <= (a.offsets ? 16 : 32) * a.E;
+  const int most = narrow ? 64 : rows_per_tile(a, pairs, blocks);
+  const int64_t count = blocks * (a.S / most + std::min(a.S, a.E));  // at least the number of tiles
+  GQ_REQUIRE(count < (int64_t(1) << 31) - 65536, "product: too many tiles");
+  const unsigned grid = unsigned(2 * std::min(pairs, std::max<int64_t>(count, 1)));
+  return narrow ? launch<64>(wmap, xmaps, a, kind, glu, most, grid, s)
+                : launch<256>(wmap, xmaps, a, kind, glu, most, grid, s);
 }
 
 }  // namespace prod

@@ -21,7 +21,7 @@ namespace slots {
 constexpr int THREADS = 1024, WARPS = THREADS / 32;
 constexpr int64_t kMaxExperts = 1024;
 constexpr int64_t kMaxChunks = 128;    // place_kernel reads every earlier chunk's counts
-constexpr int64_t kOneChunk = 4096;    // up to here one CTA sorts everything in one launch
+constexpr int64_t kOneChunk = 1024;    // up to here one CTA sorts everything in one launch (2048 slots: 9.1 us against 7.8)
 
 __host__ __device__ inline int64_t chunk_size(int64_t slots) {
   if (slots <= kOneChunk) return kOneChunk;
