@@ -39,7 +39,7 @@ namespace prod {
 namespace {
 
 constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
-constexpr int kChunk = 8;  // k-steps (64 elements each) per TMEM accumulation of the 16-bit kinds
+constexpr int kChunk = 6;  // k-steps (64 elements each) per TMEM accumulation of the 16-bit kinds
 // Registers: the drain holds a warp's 32 x 128 sums, so the other warps give it some of
 // theirs: (88 + 2 * 208) * 128 = 384 threads * 168.
 constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS), REGS_FEW = 88, REGS_DRAIN = 208;
