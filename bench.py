@@ -717,6 +717,7 @@ def run_c5(args, ws, rank, local):
             "config": {"workload": "C5 Qwen3-30B-A3B-shaped stack, MXFP4 safe-scale-search",
                        "tokens": tokens, "batch_size": args.c5_batch,
                        "experts_forward": {"grouped": "sort-based, bit-identical to the eager loop",
+                                           "fused": "sort-based, on the library's own products",
                                            "eager": "eager F.linear loop"}[args.c5_experts_forward],
                        "artifacts": "kept on the device, not written to disk"},
             "solved_elems_per_layer": elems // len(per_layer),
@@ -1040,7 +1041,7 @@ def main():
     ap.add_argument("--c5-samples", type=int, default=256)
     ap.add_argument("--c5-seqlen", type=int, default=2048)
     ap.add_argument("--c5-batch", type=int, default=16, help="c5: sequences per forward")
-    ap.add_argument("--c5-experts-forward", choices=["grouped", "eager"], default="grouped")
+    ap.add_argument("--c5-experts-forward", choices=["grouped", "fused", "eager"], default="grouped")
     ap.add_argument("--c5-dp", action="store_true",
                     help="c5: each rank forwards 1/N of the windows; Hessians summed over ranks")
     args = ap.parse_args()

@@ -86,8 +86,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--override", action="append", metavar="REGEX=BITS", help="per-tensor bit override")
     ap.add_argument("--trust-remote-code", action="store_true")
     ap.add_argument("--seed", type=int, default=17)
-    ap.add_argument("--experts-forward", default="grouped", choices=("grouped", "eager"),
-                    help="sort-based expert forward (bit-identical to the eager loop) or the eager loop")
+    ap.add_argument("--experts-forward", default="grouped", choices=("grouped", "fused", "eager"),
+                    help="sort-based expert forward (bit-identical to the eager loop), the same on this library's "
+                         "own products (SwiGLU and sums in float32; faster, equal within the loop's roundings), or "
+                         "the eager loop")
     ap.add_argument("--dp-windows", action="store_true",
                     help="with several processes: each forwards its share of the windows and Hessians are "
                          "summed over processes (the forward scales; results match one process within the "

@@ -20,6 +20,13 @@ gate/up rows are `hidden_states[tok]`: stored as token indices, not copies), the
 sorted token indices, the per-expert counts and the activation rows that feed
 down_proj (one tensor in expert order), i.e. exactly the rows the reference's
 F.linear interception stashes (capture.py:192-207), without per-expert copies.
+
+`fused_experts_forward` is the same forward on this library's own products
+(products.py): slots ordered on the device, one product with SwiGLU and one without,
+each slot's row summed per token, no host read unless a CaptureManager is active (one,
+for the counts). It captures the same rows of the same tokens; values are rounded once
+per product and once per token instead of after every elementwise step, so they agree
+with the eager loop's within its roundings, not bit for bit.
 """
 
 from __future__ import annotations
@@ -28,6 +35,8 @@ import types
 
 import torch
 import torch.nn.functional as F
+
+from . import products
 
 # expert classes whose eager forward is: gate_up = F.linear(x[tok], gate_up_proj[e]);
 # h = act_fn(gate) * up; y = F.linear(h, down_proj[e]) * w; out.index_add_(0, tok, y)
@@ -142,16 +151,47 @@ def grouped_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torc
     return out
 
 
-def install_grouped_experts(model: torch.nn.Module) -> int:
-    """Bind the sort-based forward to every supported expert module; returns how many."""
+def supports_fused(module: torch.nn.Module) -> bool:
+    """supports_grouped, and the activation is SiLU (the one the library's product applies)."""
+    act = getattr(module, "act_fn", None)
+    return supports_grouped(module) and module.gate_up_proj.shape[0] <= products.MAX_EXPERTS and (
+        act is F.silu or type(act).__name__ in ("SiLU", "SiLUActivation"))
+
+
+def fused_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
+                          top_k_weights: torch.Tensor) -> torch.Tensor:
+    """The expert forward on the library's products (bound to the module as `forward`); on
+    host tensors, and in types they do not take, the sort-based forward above."""
+    if not hidden_states.is_cuda or hidden_states.dtype not in (torch.bfloat16, torch.float16):
+        return grouped_experts_forward(self, hidden_states, top_k_index, top_k_weights)
+    sink = getattr(self, "_gq_sink", None)
+    if sink is None:
+        return products.expert_mlp(hidden_states, top_k_index, top_k_weights, self.gate_up_proj, self.down_proj)
+    T, I = hidden_states.shape[0], self.down_proj.shape[-1]
+    tok, slot, offsets = products.route_slots(top_k_index, self.gate_up_proj.shape[0])
+    counts = offsets.diff().tolist()
+    S = sum(counts)
+    h = sink.acts_out(S, T, I, hidden_states.dtype, hidden_states.device)
+    h = products.matmul_grouped(hidden_states, self.gate_up_proj, offsets, rows=tok[:S], glu=True, out=h)
+    y = products.matmul_grouped(h, self.down_proj, offsets)
+    out = products.combine_slots(y, slot, top_k_weights)
+    sink(hidden_states, tok[:S], counts, h)
+    return out
+
+
+def install_grouped_experts(model: torch.nn.Module, fused: bool = False) -> int:
+    """Bind the sort-based forward to every supported expert module; returns how many.
+    fused: the one on the library's products, where it is supported."""
     n = 0
     for m in model.modules():
         if supports_grouped(m):
-            m.forward = types.MethodType(grouped_experts_forward, m)
+            forward = fused_experts_forward if fused and supports_fused(m) else grouped_experts_forward
+            m.forward = types.MethodType(forward, m)
             n += 1
     return n
 
 
 def uses_grouped(module: torch.nn.Module) -> bool:
+    """Whether the module's rows arrive through a sort-based forward (its sink)."""
     f = module.__dict__.get("forward")
-    return getattr(f, "__func__", None) is grouped_experts_forward
+    return getattr(f, "__func__", None) in (grouped_experts_forward, fused_experts_forward)

@@ -389,7 +389,8 @@ class Pipeline:
     checkpoint_model_prefix, artifact_layers_prefix, exclude, group_size, bits,
     mode, mxfp_algorithm, damp, clip, overrides, batch_size (and optionally
     vram_gb, experts_forward: "grouped" (default; the sort-based expert forward
-    of experts.py, bit-identical to the eager loop) or "eager"). `group` is a
+    of experts.py, bit-identical to the eager loop), "fused" (the same on the
+    library's own products) or "eager"). `group` is a
     torch.distributed process group whose ranks share the solves (None: this
     process alone). Every rank runs every calibration window through each layer
     unless dp=True: then rank r forwards only its contiguous share of the windows,
@@ -416,8 +417,9 @@ class Pipeline:
         self.inner = inner
         self.layers = getattr(inner, args.layers_attr.split(".")[-1])
         self.grouped_experts = 0
-        if getattr(args, "experts_forward", "grouped") == "grouped":
-            self.grouped_experts = install_grouped_experts(model)
+        forward = getattr(args, "experts_forward", "grouped")
+        if forward in ("grouped", "fused"):
+            self.grouped_experts = install_grouped_experts(model, fused=forward == "fused")
         self.runtime_model_prefix = args.layers_attr.split(".", 1)[0]
         self.checkpoint_model_prefix = args.checkpoint_model_prefix or self.runtime_model_prefix
         self.checkpoint_layers_prefix_fmt = self._checkpoint_name(args.layers_attr) + ".{}"

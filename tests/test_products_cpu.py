@@ -79,3 +79,35 @@ def test_host_tensors_are_refused():
     for call in calls:
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_fused_forward_on_host_tensors_is_the_sort_based_one():
+    """Without a GPU the fused form falls back to the sort-based forward, bit for bit, and the
+    capture still receives its rows."""
+    from mlx_gptq_b200 import sequential
+    from mlx_gptq_b200.capture import CaptureManager
+    from mlx_gptq_b200.experts import install_grouped_experts, supports_fused, uses_grouped
+    from test_sequential_cpu import _tiny_layer
+
+    _, layer = _tiny_layer()
+    experts = layer.mlp.experts
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(40, 64, generator=g).to(torch.bfloat16)
+    w, idx = torch.softmax(torch.randn(40, 8, generator=g), -1).topk(2, dim=-1)
+    assert supports_fused(experts)
+    with torch.no_grad():
+        want = experts(x, idx, w)
+        assert install_grouped_experts(layer, fused=True) == 1 and uses_grouped(experts)
+        mgr = CaptureManager(layer, sequential.DEFAULT_EXCLUDE, 32)
+        with mgr:
+            assert torch.equal(experts(x, idx, w), want)
+    assert sum(mgr._segments["mlp.experts"].counts) == 80
+    experts.act_fn = torch.nn.GELU()
+    assert not supports_fused(experts)
+
+
+def test_command_line_accepts_the_fused_forward():
+    from mlx_gptq_b200.calibrate import build_parser
+
+    args = build_parser().parse_args(["--model", "m", "--output", "o", "--experts-forward", "fused"])
+    assert args.experts_forward == "fused"
