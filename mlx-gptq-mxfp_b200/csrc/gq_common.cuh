@@ -119,6 +119,39 @@ __device__ __forceinline__ float exp2i(int e) {
 }
 
 // ---------------------------------------------------------------------------
+// 8-bit row codes: q = rint(x / s) with an IEEE division, ties to even; |x| <= 127 s.
+// The division is done where it can matter: r = x * (1 / s) is within 127 * 2^-22 of x / s,
+// so unless r is that near a half-integer, rint(r) is the code. 0 where s is 0 or not
+// finite. Bytes of v[0 .. V) in order, packed.
+// ---------------------------------------------------------------------------
+template <int V>
+__device__ __forceinline__ void int8_codes(const float (&v)[V], float s, uint32_t (&word)[(V + 3) / 4]) {
+  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it leaves rint(r) in the low bits
+  const bool live = s > 0.0f && s < __int_as_float(0x7F800000);
+  const float inv = 1.0f / s;
+  float t[V];
+  bool near = !(inv < 1e30f);  // a subnormal scale: its reciprocal may overflow
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float r = v[i] * inv;
+    t[i] = r + kRound;
+    near |= !(fabsf(r - (t[i] - kRound)) < 0.4999f);
+  }
+  if (near && live) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = fminf(fmaxf(rintf(v[i] / s), -127.0f), 127.0f) + kRound;
+  }
+#pragma unroll
+  for (int i = 0; i < (V + 3) / 4; ++i) {
+    const uint32_t b0 = __float_as_uint(t[4 * i]), b1 = 4 * i + 1 < V ? __float_as_uint(t[4 * i + 1 < V ? 4 * i + 1 : 0]) : 0u;
+    const uint32_t b2 = 4 * i + 2 < V ? __float_as_uint(t[4 * i + 2 < V ? 4 * i + 2 : 0]) : 0u,
+                   b3 = 4 * i + 3 < V ? __float_as_uint(t[4 * i + 3 < V ? 4 * i + 3 : 0]) : 0u;
+    const uint32_t w = __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
+    word[i] = live ? w : 0u;
+  }
+}
+
+// ---------------------------------------------------------------------------
 // MXFP grids
 // ---------------------------------------------------------------------------
 

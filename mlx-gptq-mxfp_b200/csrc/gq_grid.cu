@@ -98,17 +98,12 @@ __device__ __forceinline__ void load_row_vec(const T* p, float (&v)[V]) {
 
 template <int V>
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[V], float s) {
-  int32_t c[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) c[i] = s > 0.0f ? max(-127, min(127, __float2int_rn(v[i] / s))) : 0;
-  if constexpr (V == 1) {
-    p[0] = int8_t(c[0]);
-  } else {
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < V; ++i) w[i >> 2] |= (uint32_t(c[i]) & 0xFFu) << (8 * (i & 3));
+  uint32_t w[(V + 3) / 4];
+  int8_codes<V>(v, s, w);
+  if constexpr (V == 1)
+    p[0] = int8_t(w[0]);
+  else
     *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  }
 }
 
 template <typename T, int V, int TPR, int NV>

@@ -97,13 +97,15 @@ def _row_list(rows: torch.Tensor | None, n: int) -> torch.Tensor | None:
     if rows.dim() != 1 or rows.dtype not in (torch.int32, torch.int64):
         raise ValueError("rows must be a 1-D int32 or int64 tensor")
     if rows.dtype == torch.int64:
-        rows = rows.clamp(-1, n)  # an index outside stays outside in 32 bits
-    return rows.to(torch.int32).contiguous()
+        rows = rows.clamp(-1, n).to(torch.int32)  # an index outside stays outside in 32 bits
+    return rows.contiguous()
 
 
 def _offsets(offsets: torch.Tensor, E: int, dev: torch.device) -> torch.Tensor:
     if offsets.dim() != 1 or offsets.shape[0] != E + 1 or offsets.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"offsets must be int64 [{E + 1}] (experts + 1)")
+    if offsets.dtype == torch.int64 and offsets.device == dev and offsets.is_contiguous():
+        return offsets
     return offsets.to(dev, torch.int64).contiguous()
 
 

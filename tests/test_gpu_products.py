@@ -577,3 +577,31 @@ def test_refusals():
         matmul_grouped(z(4, 16), w, off)
     with pytest.raises(RuntimeError, match="CUDA"):
         matmul_grouped(torch.zeros(4, 16, dtype=BF16), z(3, 8, 16), off)
+
+
+@pytest.mark.parametrize("rows", [2, 3000])
+def test_rtn_int8_near_ties(rows):
+    """Values at and one float32 step around every half-integer multiple of the scale: the
+    codes are those of the IEEE division (two rows go through linear_int8's own quantizer)."""
+    from mlx_gptq_b200 import linear_int8, rtn_quantize_int8
+
+    g = _gen(rows)
+    s = torch.rand(rows, 1, generator=g, device="cuda") * torch.exp(4 * _randn(g, rows, 1))
+    k = torch.arange(-127, 127, device="cuda").float() + 0.5
+    near = (k * s).double()
+    x = torch.cat([near.float(), torch.nextafter(near.float(), torch.full_like(k, 1e30).expand(rows, -1)),
+                   torch.nextafter(near.float(), torch.full_like(k, -1e30).expand(rows, -1)), 127 * s,
+                   -127 * s], 1)
+    x = torch.cat([x, torch.zeros(rows, -x.shape[1] % 16, device="cuda")], 1).contiguous()
+    q, scale = rtn_quantize_int8(x)
+    wq, ws = _codes(x)
+    assert torch.equal(scale, ws) and torch.equal(q, wq)
+    if rows == 2:
+        K = x.shape[1]
+        eye = torch.eye(K, device="cuda").to(torch.int8)
+        y = linear_int8(x, eye, torch.ones(K, device="cuda"))
+        assert torch.equal(y, wq.float() * ws[:, None])
+    tiny = x * 2.0 ** -140  # subnormal scales, and rows whose scale underflows
+    q, scale = rtn_quantize_int8(tiny)
+    wq, ws = _codes(tiny)
+    assert torch.equal(scale, ws) and torch.equal(q, wq)
