@@ -165,7 +165,8 @@ int rtn_int8(const void* X, int64_t rows, int64_t C, int64_t ldx, int8_t* q, int
   const T* x = reinterpret_cast<const T*>(X);
   const bool wide = C % 8 == 0 && Cq % 8 == 0 && ldq % 8 == 0 && ldx * int64_t(sizeof(T)) % 16 == 0 && aligned16(X) &&
                     (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
-  // 8192 rows of 4096 bf16: 2 rows per CTA of 128 threads x 4 vectors.
+  // Four vectors per thread keep enough loads in flight with few registers: 8192 rows of 4096
+  // bf16 in 29 us with 4 vectors, 31 with 2, 40 with 8; 16384 rows of 2048 in 29, 32, 39.
   auto run = [&](auto v, auto tpr, auto nv) {
     constexpr int V = decltype(v)::value, TPR = decltype(tpr)::value, NV = decltype(nv)::value;
     return launch_dependent("rtn_int8_kernel", rtn_int8_kernel<T, V, TPR, NV>,
@@ -177,11 +178,13 @@ int rtn_int8(const void* X, int64_t rows, int64_t C, int64_t ldx, int8_t* q, int
   constexpr std::integral_constant<int, 4> four{};
   constexpr std::integral_constant<int, 8> eight{};
   constexpr std::integral_constant<int, 32> warp{};
+  constexpr std::integral_constant<int, 64> quarter{};
   constexpr std::integral_constant<int, 128> half{};
   constexpr std::integral_constant<int, 256> cta{};
   if (!wide) return Cq <= 256 ? run(one, warp, eight) : run(one, cta, eight);
   if (Cq <= 512) return run(eight, warp, two);
   if (Cq <= 1024) return run(eight, warp, four);
+  if (Cq <= 2048) return run(eight, quarter, four);
   if (Cq <= 4096) return run(eight, half, four);
   if (Cq <= 8192) return run(eight, cta, four);
   return run(eight, cta, eight);

@@ -605,3 +605,112 @@ def test_rtn_int8_near_ties(rows):
     q, scale = rtn_quantize_int8(tiny)
     wq, ws = _codes(tiny)
     assert torch.equal(scale, ws) and torch.equal(q, wq)
+
+
+def test_outputs_and_weights_past_32_bits():
+    """More than 2^31 elements in the output, and in the weights with rows for the last expert
+    only: every offset is 64 bits wide."""
+    from mlx_gptq_b200 import matmul_grouped, matmul_int8
+
+    g = _gen(3)
+    S, N, K = 70000, 32768, 16
+    x, w = _randn(g, S, K).to(BF16), _randn(g, 1, N, K).to(BF16)
+    off = torch.tensor([0, S], device="cuda")
+    for engine in ENGINES:
+        y = matmul_grouped(x, w, off, engine=engine)
+        for rows in (slice(0, 3), slice(S // 2, S // 2 + 3), slice(S - 3, S)):
+            want, err = _reference(x[rows].double(), w.double(), (3,), torch.arange(3, device="cuda"), False, 3)
+            _assert_close(y[rows], want, err, engine)
+        del y
+    one = torch.ones(1, device="cuda")
+    xq = torch.randint(-127, 128, (S, K), generator=g, device="cuda", dtype=torch.int8)
+    wq = torch.randint(-127, 128, (N, K), generator=g, device="cuda", dtype=torch.int8)
+    y = matmul_int8(xq, one.expand(S), wq, one.expand(N))
+    want = (xq[-2:].double() @ wq.double().t())
+    _assert_close(y[-2:], want, torch.zeros_like(want))
+    del y
+    E, N, K = 120, 8192, 2304  # 2.26e9 weights
+    w = torch.zeros(E, N, K, dtype=BF16, device="cuda")
+    w[-1] = (_randn(g, N, K) * 0.1).to(BF16)
+    counts = [0] * (E - 1) + [70]
+    x = _randn(g, 70, K).to(BF16)
+    want, err = _reference(x.double(), w[-1:].double(), (70,), torch.arange(70, device="cuda"), True, 70)
+    for engine in ENGINES:
+        _assert_close(matmul_grouped(x, w, _offsets(counts), glu=True, engine=engine), want, err, engine)
+
+
+def test_results_do_not_depend_on_the_call():
+    """The same call again, in a batch of calls, through a row list that changes nothing and
+    with weights that are not neighbours in memory: the same bits."""
+    from mlx_gptq_b200 import matmul_grouped, matmul_grouped_int8, rtn_quantize_int8
+
+    g = _gen(4)
+    counts = (300, 0, 77, 1, 512)
+    S, K, N = sum(counts), 320, 192
+    x, w = _randn(g, S, K).to(F16), (_randn(g, 5, N, K) * 0.1).to(F16)
+    off, every = _offsets(counts), torch.arange(S, device="cuda")
+    apart = torch.zeros(5, N + 8, K + 16, dtype=F16, device="cuda")
+    apart[:, 8:, 8:8 + K] = w
+    (xq, xs), (wq, ws) = rtn_quantize_int8(x), rtn_quantize_int8(w)
+    for engine in ENGINES:
+        y = matmul_grouped(x, w, off, glu=True, engine=engine)
+        assert all(torch.equal(y, matmul_grouped(x, w, off, glu=True, engine=engine)) for _ in range(5))
+        assert torch.equal(y, matmul_grouped(x, w, off, rows=every, glu=True, engine=engine))
+        assert torch.equal(y, matmul_grouped(x, apart[:, 8:, 8:8 + K], off, glu=True, engine=engine))
+        # an expert's rows do not depend on the others
+        alone = matmul_grouped(x[300:377], w[2:3], _offsets((77,)), glu=True, engine=engine)
+        assert torch.equal(alone, y[300:377])
+        z = matmul_grouped_int8(xq, xs, wq, ws, off, glu=True, engine=engine)
+        assert torch.equal(z, matmul_grouped_int8(xq, xs, wq, ws, off, rows=every, glu=True, engine=engine))
+    # 8-bit sums are exact: both kernels round the same numbers
+    assert torch.equal(*(matmul_grouped_int8(xq, xs, wq, ws, off, out_dtype=F32, engine=e) for e in ENGINES))
+
+
+@pytest.mark.parametrize("T", [1, 5, 300])
+def test_expert_mlp_does_not_read_what_nothing_routes(T):
+    """Unrouted experts' weights, dropped positions' weights and rows behind the last slot may
+    hold anything."""
+    from mlx_gptq_b200 import combine_slots, expert_mlp
+
+    g = _gen(T)
+    E, k, C, I = 12, 3, 96, 48
+    x = _randn(g, T, C).to(BF16)
+    gate_up, down = (_randn(g, E, 2 * I, C) * 0.1).to(BF16), (_randn(g, E, C, I) * 0.1).to(BF16)
+    idx = torch.randint(0, E - 2, (T, k), generator=g, device="cuda")
+    idx[:, 1] = torch.where(idx[:, 1] % 2 == 0, -1, idx[:, 1])
+    wt = torch.rand(T, k, generator=g, device="cuda")
+    want = expert_mlp(x, idx, wt, gate_up, down)
+    gate_up[-2:], down[-2:] = float("nan"), float("inf")
+    wt = torch.where(idx < 0, float("nan"), wt)
+    acts = torch.full((T * k, I), float("nan"), dtype=BF16, device="cuda")
+    assert torch.equal(want, expert_mlp(x, idx, wt, gate_up, down, acts=acts))
+    y = torch.full((4, 8), float("inf"), dtype=BF16, device="cuda")
+    y[1] = 1
+    slot = torch.tensor([[1, -1, 4]], dtype=torch.int32, device="cuda")
+    w = torch.tensor([[2.0, float("nan"), float("inf")]], device="cuda")
+    assert combine_slots(y, slot, w).tolist() == [[2.0] * 8]
+
+
+def test_swiglu_over_its_range():
+    """Gates from -1e4 to 1e4 (and the infinities): silu neither overflows nor loses its sign."""
+    from mlx_gptq_b200 import matmul_grouped
+
+    gates = torch.cat([torch.linspace(-120, 120, 241), torch.tensor([-1e4, -300.0, 300.0, 1e4])]).cuda()
+    n = gates.shape[0]
+    x = torch.zeros(n, 16, dtype=BF16, device="cuda")
+    x[:, 0], x[:, 1] = gates.to(BF16), 1.0
+    w = torch.zeros(1, 2, 16, dtype=BF16, device="cuda")
+    w[0, 0, 0], w[0, 1, 1] = 1.0, 2.0  # gate = x0, up = 2
+    g = x[:, 0].double()
+    want = (2 * torch.where(g >= 0, g / (1 + torch.exp(-g)), g * torch.exp(g) / (1 + torch.exp(g))))[:, None]
+    # 8 float32 steps; below 2^-126 results may be subnormal
+    err = 8 * 2.0 ** -23 * want.abs() + 2.0 ** -126
+    for engine in ENGINES:
+        y = matmul_grouped(x, w, _offsets((n,)), glu=True, engine=engine)
+        u = 2.0 ** -8
+        assert bool(((y.double() - want).abs() <= err + u * (want.abs() + err) + 2.0 ** -134).all())
+    x[0, 0], x[1, 0], x[2, 0] = float("inf"), float("-inf"), float("nan")
+    for engine in ENGINES:
+        # inf * 0 of the other terms makes the sums NaN, as in any product
+        y = matmul_grouped(x, w, _offsets((n,)), glu=True, engine=engine)
+        assert not bool(torch.isfinite(y[:3]).any()) and bool(torch.isfinite(y[3:]).all())
