@@ -13,7 +13,7 @@
 // the weights and half of the rows per 128-byte k-step. Persistent: pair p takes tiles p,
 // p + pairs, ... of a list that every role derives from the offsets on the device (tiles
 // per expert, scanned once into shared memory): nothing is read back to the host.
-//   warp 0       TMA: weights [expert, channel, k] and X
+//   warps 0, 2   TMA: weights [expert, channel, k]; rows of X
 //   warp 1       MMA issuer (even CTA) into one of two TMEM accumulator sets
 //   warps 4-11   drain the other set into registers; scale / bias / SwiGLU, round once, store
 // A row list is applied by a copy before the launch (gather_kernel). Gathering inside the
@@ -327,7 +327,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                  "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
-  grid_wait();  // the barriers and TMEM above were set up while the kernel before ended
+  if (!a.early) grid_wait();  // the barriers and TMEM above were set up while the kernel before ended
   if (warp == 2) {
     // Rows of every expert and the exclusive scan of their tiles. Offsets that run backwards
     // are raised to the largest before them, so that the tiles stay within S rows whatever
@@ -363,8 +363,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   cluster_sync();
-  grid_release();
   tc_fence_after();
+  if (warp != 0) {  // the weights' thread goes ahead
+    if (a.early) grid_wait();
+    grid_release();
+  }
   const uint32_t tmem = *tmem_slot;
   const int tiles = ex.first_tile[E] * ct;  // below 2^31: checked by the host for any offsets
 
@@ -449,31 +452,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
     if (warp == 0 && lane == 0) {
+      // The weights, and the announcement of both CTAs' bytes. Never waits for the rows: with
+      // early the stages fill with weights while the kernel before ends.
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
-      for (int b = 0; b < X_MAPS; ++b)
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&xmaps.box[b])) : "memory");
       Ring ring;
       bool ok = true, lapped = false;
       for (int q = pair; q < tiles && ok; q += pairs) {
         const Tile t = tile_of(q, ex, E, ct, STEP, most);
-        const int half = t.n / 2, x_rows = (half + 15) / 16 * 16;  // <= 128
-        const uint32_t bytes = A_BYTES + uint32_t(x_rows) * 128;
-        const int ch = (t.block * 2 + int(rank)) * (GLU ? 64 : 128), y = int(t.row0) + int(rank) * half;
+        const uint32_t bytes = 2 * (A_BYTES + uint32_t((t.n / 2 + 15) / 16 * 16) * 128);
+        const int ch = (t.block * 2 + int(rank)) * (GLU ? 64 : 128);
         for (int kt = 0; kt < KT; ++kt) {
           const int s = ring.stage;
           if (!mbar_wait(&empty[s], ring.phase ^ 1, abort_flag, a.status)) {
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * bytes);  // both CTAs' bytes
-          uint8_t* st = smem + s * STAGE_BYTES;
-          tma_4d(st, &wmap, kt * KSTEP, 0, ch, t.expert, &full[s]);  // (k, gate / up, channel, expert)
-          // few large boxes: each costs the TMA unit and this thread a fixed time
-          for (int b = 0, r = 0; b < X_MAPS; ++b)
-            if (x_rows & (128 >> b)) {
-              tma_2d(st + A_BYTES + r * 128, &xmaps.box[b], kt * KSTEP, y + r, &full[s]);
-              r += 128 >> b;
-            }
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+          tma_4d(smem + s * STAGE_BYTES, &wmap, kt * KSTEP, 0, ch, t.expert, &full[s]);  // (k, gate / up, channel, expert)
           ring.step(STAGES);
           lapped |= ring.stage == 0;
         }
@@ -483,6 +478,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         for (int i = 0; i < STAGES; ++i)  // the last load of stage i: this lap's, or the lap's before
           if (i < ring.stage || lapped)
             mbar_wait(&full[i], i < ring.stage ? ring.phase : ring.phase ^ 1, &never, nullptr);
+      }
+    } else if (warp == 2 && lane == 0) {
+      // The rows, by a thread of their own: issuing both loads from one costs 5%.
+      for (int b = 0; b < X_MAPS; ++b)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&xmaps.box[b])) : "memory");
+      Ring ring;
+      bool ok = true;
+      for (int q = pair; q < tiles && ok; q += pairs) {
+        const Tile t = tile_of(q, ex, E, ct, STEP, most);
+        const int half = t.n / 2, x_rows = (half + 15) / 16 * 16;  // <= 128
+        const int y = int(t.row0) + int(rank) * half;
+        for (int kt = 0; kt < KT; ++kt) {
+          const int s = ring.stage;
+          if (!mbar_wait(&empty[s], ring.phase ^ 1, abort_flag, a.status)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * STAGE_BYTES + A_BYTES;
+          // few large boxes: each costs the TMA unit and this thread a fixed time
+          for (int b = 0, r = 0; b < X_MAPS; ++b)
+            if (x_rows & (128 >> b)) {
+              tma_2d(st + r * 128, &xmaps.box[b], kt * KSTEP, y + r, &full[s]);
+              r += 128 >> b;
+            }
+          ring.step(STAGES);
+        }
       }
     } else if (warp == 1 && lane == 0 && rank == 0) {
       Ring ring;
@@ -605,7 +626,8 @@ int rows_per_tile(const Args& a, int64_t pairs, int64_t blocks) {
 
 }  // namespace
 
-int launch_tc(const Args& a, Kind kind, bool glu, void* gathered, cudaStream_t s) {
+int launch_tc(const Args& args, Kind kind, bool glu, void* gathered, cudaStream_t s) {
+  Args a = args;
   int dev = 0, sms = 0;
   GQ_CUDA_TRY(cudaGetDevice(&dev));
   GQ_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
@@ -627,6 +649,7 @@ int launch_tc(const Args& a, Kind kind, bool glu, void* gathered, cudaStream_t s
     st = launch_dependent("gather_kernel", gather_kernel, dim3(unsigned((warps + 7) / 8)), 256, 0, s, a,
                           reinterpret_cast<uint4*>(gathered), row_bytes / 16);
     if (st != GQ_OK) return st;
+    a.early = 1;  // W and offsets are older than the copy
   }
   for (int b = 0; b < X_MAPS; ++b) {
     const cuuint64_t xdims[2] = {cuuint64_t(a.K), cuuint64_t(a.rows ? a.S : a.n_src)};
