@@ -71,7 +71,6 @@ __device__ __forceinline__ uint32_t cta_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint32_t even_cta(const void* p) { return smem_u32(p) & kEvenCta; }
 
 // Arrive on a barrier of the even CTA, releasing this thread's writes to the cluster.
 __device__ __forceinline__ void arrive_even(uint64_t* bar) {
@@ -79,35 +78,52 @@ __device__ __forceinline__ void arrive_even(uint64_t* bar) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(r) : "memory");
 }
-// mbar_wait for barriers that the other CTA of the pair arrives on.
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                             int32_t* status) {
+// Waits on a barrier given by its address; the first try is inline, the bounded loop is not.
+// CLUSTER: the other CTA of the pair arrives on it, and its writes are acquired.
+__device__ __noinline__ bool wait_slowly(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+  return mbar_wait(reinterpret_cast<uint64_t*>(__cvta_shared_to_generic(bar)), parity, abort_flag, status);
+}
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
   uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
+  if constexpr (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
   if (ok) return true;
-  if (!mbar_wait(bar, parity, abort_flag, status)) return false;
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  if (!wait_slowly(bar, parity, abort_flag, status)) return false;
+  if (CLUSTER) asm volatile("fence.acq_rel.cluster;" ::: "memory");
   return true;
 }
 
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+__device__ __forceinline__ void expect_tx_at(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// TMA loads into dst, announced on bar of the even CTA (shared-memory addresses).
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-      "[%4];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(even_cta(bar))
+      "[%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar & kEvenCta)
       : "memory");
 }
-__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-      "%4, %5}], [%6];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(even_cta(bar))
+      "%4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar & kEvenCta)
       : "memory");
 }
 
@@ -129,10 +145,10 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
         : "memory");
 }
 // Arrives on the barrier at this offset in both CTAs once the issued MMAs complete.
-__device__ __forceinline__ void commit(uint64_t* bar) {
+__device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
+          bar),
       "h"(uint16_t(3))
       : "memory");
 }
@@ -144,14 +160,22 @@ __device__ __forceinline__ uint32_t instruction_desc(Kind kind, int n) {
   return types | (uint32_t(n >> 3) << 17) | (uint32_t(256 >> 4) << 24);
 }
 
-// Position in the stage ring. The waits it stands for are on the critical path of one
-// thread each: no division per step (64-bit remainders cost 15% of the whole kernel).
+// Position in the stage ring, as the shared-memory addresses of the stage and its barriers.
+// The loops over it run on one thread each and bound the kernel when they are long: no
+// division, no address arithmetic beyond a step (64-bit remainders cost 15% here, one
+// thread for both operands' loads 5%).
+template <int STAGES, uint32_t STAGE_BYTES>
 struct Ring {
-  int stage = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void step(int stages) {
-    if (++stage == stages) stage = 0, phase ^= 1;
+  uint32_t data, bar, phase = 0;  // stage s: data + s * STAGE_BYTES; bar: its full, bar + 8 * STAGES: its empty barrier
+  uint32_t data0, end;
+  __device__ __forceinline__ Ring(const uint8_t* smem, const uint64_t* full)
+      : data(smem_u32(smem)), bar(smem_u32(full)), data0(data), end(data + STAGES * STAGE_BYTES) {}
+  __device__ __forceinline__ void step() {
+    data += STAGE_BYTES, bar += 8;
+    if (data == end) data = data0, bar -= 8 * STAGES, phase ^= 1;
   }
+  __device__ __forceinline__ uint32_t full() const { return bar; }
+  __device__ __forceinline__ uint32_t empty() const { return bar + 8 * STAGES; }
 };
 
 struct XMaps {
@@ -455,88 +479,88 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       // The weights, and the announcement of both CTAs' bytes. Never waits for the rows: with
       // early the stages fill with weights while the kernel before ends.
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&wmap)) : "memory");
-      Ring ring;
-      bool ok = true, lapped = false;
+      Ring<STAGES, STAGE_BYTES> ring(smem, full);
+      int64_t loads = 0;
+      bool ok = true;
       for (int q = pair; q < tiles && ok; q += pairs) {
         const Tile t = tile_of(q, ex, E, ct, STEP, most);
         const uint32_t bytes = 2 * (A_BYTES + uint32_t((t.n / 2 + 15) / 16 * 16) * 128);
         const int ch = (t.block * 2 + int(rank)) * (GLU ? 64 : 128);
         for (int kt = 0; kt < KT; ++kt) {
-          const int s = ring.stage;
-          if (!mbar_wait(&empty[s], ring.phase ^ 1, abort_flag, a.status)) {
+          if (!wait_at<false>(ring.empty(), ring.phase ^ 1, abort_flag, a.status)) {
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-          tma_4d(smem + s * STAGE_BYTES, &wmap, kt * KSTEP, 0, ch, t.expert, &full[s]);  // (k, gate / up, channel, expert)
-          ring.step(STAGES);
-          lapped |= ring.stage == 0;
+          if (rank == 0) expect_tx_at(ring.full(), bytes);
+          tma_4d(ring.data, &wmap, kt * KSTEP, 0, ch, t.expert, ring.full());  // (k, gate / up, channel, expert)
+          ring.step();
+          ++loads;
         }
       }
       if (*abort_flag && rank == 0) {  // let copies already in flight land before the CTA exits
         volatile int never = 0;
-        for (int i = 0; i < STAGES; ++i)  // the last load of stage i: this lap's, or the lap's before
-          if (i < ring.stage || lapped)
-            mbar_wait(&full[i], i < ring.stage ? ring.phase : ring.phase ^ 1, &never, nullptr);
+        for (int64_t i = loads > STAGES ? loads - STAGES : 0; i < loads; ++i)
+          mbar_wait(&full[i % STAGES], (i / STAGES) & 1, &never, nullptr);
       }
     } else if (warp == 2 && lane == 0) {
       // The rows, by a thread of their own: issuing both loads from one costs 5%.
       for (int b = 0; b < X_MAPS; ++b)
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&xmaps.box[b])) : "memory");
-      Ring ring;
+      Ring<STAGES, STAGE_BYTES> ring(smem, full);
       bool ok = true;
       for (int q = pair; q < tiles && ok; q += pairs) {
         const Tile t = tile_of(q, ex, E, ct, STEP, most);
         const int half = t.n / 2, x_rows = (half + 15) / 16 * 16;  // <= 128
         const int y = int(t.row0) + int(rank) * half;
+        // few large boxes: the largest that fits, and what is left
+        int first = 0;
+        while (x_rows < (128 >> first)) ++first;
+        const CUtensorMap* map = &xmaps.box[first];
+        const int left = x_rows - (128 >> first);
         for (int kt = 0; kt < KT; ++kt) {
-          const int s = ring.stage;
-          if (!mbar_wait(&empty[s], ring.phase ^ 1, abort_flag, a.status)) {
+          if (!wait_at<false>(ring.empty(), ring.phase ^ 1, abort_flag, a.status)) {
             ok = false;
             break;
           }
-          uint8_t* st = smem + s * STAGE_BYTES + A_BYTES;
-          // few large boxes: each costs the TMA unit and this thread a fixed time
-          for (int b = 0, r = 0; b < X_MAPS; ++b)
-            if (x_rows & (128 >> b)) {
-              tma_2d(st + r * 128, &xmaps.box[b], kt * KSTEP, y + r, &full[s]);
-              r += 128 >> b;
-            }
-          ring.step(STAGES);
+          tma_2d(ring.data + A_BYTES, map, kt * KSTEP, y, ring.full());
+          if (left)
+            for (int b = first + 1, r = 128 >> first; b < X_MAPS; ++b)
+              if (left & (128 >> b)) {
+                tma_2d(ring.data + A_BYTES + r * 128, &xmaps.box[b], kt * KSTEP, y + r, ring.full());
+                r += 128 >> b;
+              }
+          ring.step();
         }
       }
     } else if (warp == 1 && lane == 0 && rank == 0) {
-      Ring ring;
+      Ring<STAGES, STAGE_BYTES> ring(smem, full);
       int n_chunk = 0;
       bool ok = true;
-      const uint64_t desc = umma_desc_sw128(smem_u32(smem), 16, 1024);  // + (byte offset >> 4)
+      const uint64_t desc = umma_desc_sw128(0, 16, 1024);  // + (address >> 4)
       for (int q = pair; q < tiles && ok; q += pairs) {
         const Tile t = tile_of(q, ex, E, ct, STEP, most);
         const uint32_t idesc = instruction_desc(kind, t.n);
         for (int k0 = 0; k0 < KT && ok; k0 += chunk, ++n_chunk) {
           const int buf = n_chunk & 1, k1 = k0 + chunk < KT ? k0 + chunk : KT;
-          if (!wait_cluster(&tempty[buf], ((n_chunk >> 1) & 1) ^ 1, abort_flag, a.status)) {
+          if (!wait_at<true>(smem_u32(&tempty[buf]), ((n_chunk >> 1) & 1) ^ 1, abort_flag, a.status)) {
             ok = false;
             break;
           }
           const uint32_t d = tmem + uint32_t(buf * 256);
           for (int kt = k0; kt < k1; ++kt) {
-            const int s = ring.stage;
-            if (!wait_cluster(&full[s], ring.phase, abort_flag, a.status)) {
+            if (!wait_at<true>(ring.full(), ring.phase, abort_flag, a.status)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint64_t ad = desc + uint32_t(s) * (STAGE_BYTES >> 4), bd = ad + (A_BYTES >> 4);
+            const uint64_t ad = desc + (ring.data >> 4), bd = ad + (A_BYTES >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {  // 32 bytes of k each, inside the 128-byte swizzle atom
-              const uint32_t more = kt != k0 || kk != 0;
-              mma<I8>(d, ad + 2 * kk, bd + 2 * kk, idesc, more);
-            }
-            commit(&empty[s]);  // frees the stage once these MMAs have read it
-            ring.step(STAGES);
+            for (int kk = 0; kk < 4; ++kk)  // 32 bytes of k each, inside the 128-byte swizzle atom
+              mma<I8>(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0 || kt != k0);
+            commit(ring.empty());  // frees the stage once these MMAs have read it
+            ring.step();
           }
-          if (ok) commit(&tfull[buf]);
+          if (ok) commit(smem_u32(&tfull[buf]));
         }
       }
     }
