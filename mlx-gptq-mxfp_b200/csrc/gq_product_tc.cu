@@ -39,7 +39,8 @@ namespace prod {
 namespace {
 
 constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
-constexpr int kChunk = 6;  // k-steps (64 elements each) per TMEM accumulation of the 16-bit kinds
+// k-steps (64 elements each) per TMEM accumulation of the 16-bit kinds, see above
+constexpr int kChunk = 16, kChunkGlu = 7;
 // Registers: the drain holds a warp's 32 x 128 sums, so the other warps give it some of
 // theirs: (88 + 2 * 208) * 128 = 384 threads * 168.
 constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS), REGS_FEW = 88, REGS_DRAIN = 208;
@@ -332,7 +333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const int64_t I = GLU ? a.N / 2 : a.N;
   const int ct = int((I + (GLU ? 127 : 255)) / (GLU ? 128 : 256));  // channel blocks
   const int KT = int((a.K + KSTEP - 1) / KSTEP);
-  const int chunk = I8 ? KT : kChunk;  // k-steps per accumulation
+  const int chunk = I8 ? KT : (GLU ? kChunkGlu : kChunk);  // k-steps per accumulation
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
