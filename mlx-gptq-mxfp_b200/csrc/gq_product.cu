@@ -10,10 +10,11 @@ namespace {
 // The few-rows kernel streams the weights with any number of channel blocks and reads them
 // again (from L2) for every 8 .. 32 rows; the tcgen05 kernel reads them once per 64 .. 256
 // rows but has only CTA pairs x 256 channels to spread them over. Measured, 128 experts of
-// [1536, 2048] with SwiGLU, 128 rows: 46 against 54 us, 512 rows: 95 against 77 us; dense
-// s8 [4096, 4096], 64 rows: 13 against 19 us, 128 rows: 24 against 20 us.
+// [1536, 2048] with SwiGLU and of [2048, 768], both: 64 rows 61 against 66 us, 128 rows 85
+// against 78, 512 rows 191 against 112; dense s8 [4096, 4096], 64 rows 13 against 16 us,
+// 128 rows 23 against 16.
 bool by_rows(int64_t S, int64_t E, int engine) {
-  return engine == 0 || (engine < 0 && S <= (E == 1 ? 64 : E));
+  return engine == 0 || (engine < 0 && S <= (E == 1 ? 64 : (E + 1) / 2));
 }
 
 int check(const char* what, const Args& a, Kind kind, bool glu, int engine) {

@@ -17,17 +17,24 @@
 //   warp 1       MMA issuer (even CTA) into one of two TMEM accumulator sets
 //   warps 4-11   drain the other set into registers; scale / bias / SwiGLU, round once, store
 // A row list is applied by a copy before the launch (gather_kernel). Gathering inside the
-// kernel, six warps with cp.async beside the TMA producer, was built and measured: 541 us
-// against 457 + 55 us for 65536 rows of K = 2048 times 128 experts of 1536 channels.
+// kernel was built and measured on 8192 x 4096 x 4096 bf16, 184 us without and 204 us with
+// the copy: 262 us with cp.async by six warps into the stages, 284 us with gather4 loads
+// issued by six threads (20 ns each, 32 per stage).
 //
-// What bounds it: with 256 x 256 tiles every SM takes 32 KB per 512 cycles of MMA; the
-// loads alone sustain 47 bytes per cycle and SM (13 TB/s from L2 over the GPU), 690 cycles.
+// What bounds it, on the same product: the loads alone take 135 us (59 bytes per cycle and
+// SM, 32 KB per stage), the MMAs alone 124 us at 1.85 GHz, together 178 us with one
+// accumulation per tile: both use shared memory's bandwidth. cuBLAS takes 178 us.
 //
 // Precision: a tensor-core step loses up to a float32 step of the partial sum, always
 // toward zero, so one accumulator over K = 2048 drifts by 5e-6 of |y| (8 x a float32 FMA
-// chain). The 16-bit kinds therefore accumulate kChunk k-steps in TMEM and add the chunks
-// in registers, rounding to nearest (the same remedy as in gq_hessian.cu); s32 sums are
-// exact and take one chunk per tile.
+// chain). The 16-bit kinds therefore leave TMEM every kChunk k-steps and add the chunks in
+// registers, rounding to nearest (the same remedy as in gq_hessian.cu): 1024 products, which
+// keeps the drift 30 times below an f16 output's rounding and costs 3%. Before SwiGLU, whose
+// rows are operands again, sums stay as near as an FMA chain's: with L k-steps per chunk the
+// drift is proportional to L |y|, the chain's rounding grows with sqrt(K) at most, so L is 7 at
+// K = 2048 (1.3 x the chain's error, for 12% of the time: a drain of the accumulator takes
+// 0.3 us from the MMAs), grows with sqrt(K) above and shrinks with K below. s32 sums are
+// exact: one accumulation per tile.
 // Every wait is bounded (gq_common.cuh); a wait that gives up records GQ_ERR_TIMEOUT.
 #include <algorithm>
 #include <type_traits>
@@ -40,7 +47,10 @@ namespace {
 
 constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
 // k-steps (64 elements each) per TMEM accumulation of the 16-bit kinds, see above
-constexpr int kChunk = 16, kChunkGlu = 7;
+constexpr int kChunk = 16;
+__device__ __forceinline__ int chunk_glu(int steps) {
+  return steps > 32 ? __float2int_rn(sqrtf(1.5f * float(steps))) : max(2, (7 * steps + 16) / 32);
+}
 // Registers: the drain holds a warp's 32 x 128 sums, so the other warps give it some of
 // theirs: (88 + 2 * 208) * 128 = 384 threads * 168.
 constexpr int THREADS = 32 * (EPI_WARP0 + EPI_WARPS), REGS_FEW = 88, REGS_DRAIN = 208;
@@ -51,8 +61,9 @@ constexpr uint32_t kEvenCta = 0xFEFFFFFFu;  // shared::cluster address -> even C
 
 // Two tile widths. 256 rows for throughput. 64 rows where experts have few (decoding
 // batches): the time is then that of streaming the weights, a tile's loads are nearly all
-// weights, and 10 stages of 20 KB keep 160 KB of them in flight per SM where 6 of 32 KB
-// keep 96.
+// weights, and 10 stages of 20 KB keep more of them in flight than 6 of 32 KB. 128 experts
+// of [1536, 2048] and [2048, 768], 64 tokens x 8: 112 against 118 us for both products; 256
+// tokens: 171 against 165.
 template <int NMAX>
 struct Shape {
   static constexpr uint32_t B_BYTES = uint32_t(NMAX / 2) * 128;
@@ -333,7 +344,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const int64_t I = GLU ? a.N / 2 : a.N;
   const int ct = int((I + (GLU ? 127 : 255)) / (GLU ? 128 : 256));  // channel blocks
   const int KT = int((a.K + KSTEP - 1) / KSTEP);
-  const int chunk = I8 ? KT : (GLU ? kChunkGlu : kChunk);  // k-steps per accumulation
+  const int chunk = I8 ? KT : (GLU ? chunk_glu(KT) : kChunk);  // k-steps per accumulation
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -632,10 +643,10 @@ __global__ void __launch_bounds__(256) gather_kernel(const Args a, uint4* __rest
 }
 
 // Rows per tile. Grouped: 256, the counts are on the device. Dense: the number of row tiles
-// whose last round of tiles over the CTA pairs is filled best; a k-step of a tile of n rows
-// takes the loads of 128 channels and n / 2 rows (128 bytes each, 47 bytes per cycle), so
-// a round costs 16384 + 64 n. 1357 rows x 4096 channels: 96 tiles of 240 rows on 74
-// pairs are two rounds, 144 tiles of 160 rows are two shorter ones.
+// whose rounds over the CTA pairs cost least, a round of tiles of n rows being taken as the
+// bytes that a k-step of such a tile loads per SM, 128 channels and n / 2 rows of 128 bytes.
+// 1357 rows x 4096 channels: 96 tiles of 240 rows on 74 pairs are two rounds, 144 tiles of
+// 160 rows two shorter ones (K = 11008, s8: 78 against 91 us).
 int rows_per_tile(const Args& a, int64_t pairs, int64_t blocks) {
   if (a.offsets) return 256;
   int best = 256;
@@ -684,7 +695,7 @@ int launch_tc(const Args& args, Kind kind, bool glu, void* gathered, cudaStream_
     if (st != GQ_OK) return st;
   }
   const int64_t pairs = std::max(sms / 2, 1), blocks = (a.N + 255) / 256;
-  const bool narrow = a.S <= (a.offsets ? 16 : 32) * a.E;
+  const bool narrow = a.S <= (a.offsets ? 8 : 32) * a.E;
   const int most = narrow ? 64 : rows_per_tile(a, pairs, blocks);
   const int64_t count = blocks * (a.S / most + std::min(a.S, a.E));  // at least the number of tiles
   GQ_REQUIRE(count < (int64_t(1) << 31) - 65536, "product: too many tiles");
