@@ -319,7 +319,7 @@ int gq_combine_slots(const void* y, int dtype, int64_t S, int64_t ldy, const int
  * followed out of bounds); nullable with E = 1: all S rows. W: [E, N, K], strides ldw per
  * channel and stride_w per expert. Y: [S, N] ([S, I] with glu), row stride ldy; rows from
  * offsets[E] on are written as zeros with zero_behind != 0, else left as they were.
- * K, ldx, ldw, stride_w multiples of 8, X and W 16-byte aligned; E <= 1024.
+ * K, ldx, ldw, stride_w multiples of 8, X and W 16-byte aligned; E <= 1024, S <= 2^30.
  * engine: -1 chosen by sizes, 0 the few-rows kernel, 1 the tcgen05 kernel.
  * workspace: needed with rows, where the tcgen05 kernel runs (the rows are gathered into
  * it first): gq_matmul_workspace_size bytes, 16-byte aligned; 0: none.

@@ -20,8 +20,8 @@ bool by_rows(int64_t S, int64_t E, int engine) {
 int check(const char* what, const Args& a, Kind kind, bool glu, int engine) {
   const int64_t es = kind == S8 ? 1 : 2;
   const int64_t I = glu ? a.N / 2 : a.N;
-  GQ_REQUIRE(a.S >= 0 && a.S < (int64_t(1) << 31) && a.n_src >= 0 && a.n_src < (int64_t(1) << 31),
-             "%s: %lld rows of %lld", what, (long long)a.S, (long long)a.n_src);
+  GQ_REQUIRE(a.S >= 0 && a.S <= (int64_t(1) << 30) && a.n_src >= 0 && a.n_src < (int64_t(1) << 31),
+             "%s: %lld rows of %lld, at most 2^30 of 2^31 - 1", what, (long long)a.S, (long long)a.n_src);
   GQ_REQUIRE(a.E >= 1 && a.E <= kMaxExperts, "%s: %lld experts, at most %lld", what, (long long)a.E,
              (long long)kMaxExperts);
   GQ_REQUIRE(a.N >= 1 && a.N < (int64_t(1) << 31) && a.K >= 1 && a.K < (int64_t(1) << 31), "%s: sizes", what);

@@ -7,7 +7,7 @@ Here:
 * ``route_slots`` / ``combine_slots``: the order of a top-k routing's slots by expert,
   and the weighted sum of the slots' rows per token;
 * ``matmul_grouped``: rows of every expert times that expert's weights, ragged sizes,
-  rows optionally taken through a row list, SwiGLU optionally applied, one launch;
+  rows optionally taken through a row list, SwiGLU optionally applied;
 * ``expert_mlp``: the expert MLP of a routed batch from the three above;
 * ``matmul_int8`` / ``matmul_grouped_int8`` / ``linear_int8``: the same products on 8-bit
   codes with one scale per row and one per channel (codes from
@@ -16,6 +16,9 @@ Here:
 All run on the tensors' CUDA device and its current stream and never wait for the
 device, so they can be captured into a CUDA graph (after one ordinary call per device).
 They have no backward: with gradients enabled, inputs that require them are refused.
+The tensor-core kernel's waits are bounded like the Hessian's: one that gives up leaves
+GQ_ERR_TIMEOUT in the device's status word, which _lib.raise_on_device_timeout reads (and
+every solver before it uses a Hessian).
 """
 
 from __future__ import annotations

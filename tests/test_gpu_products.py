@@ -518,6 +518,10 @@ def test_empty_calls():
     assert not bool(combine_slots(z(0, 8), z(3, 2, dt=torch.int32) - 1, z(3, 2, dt=F32) + 1).any())
     assert matmul_grouped(z(0, 16), z(6, 8, 16), offsets).shape == (0, 8)
     assert expert_mlp(z(0, 16), z(0, 4, dt=torch.int64), z(0, 4, dt=F32), z(6, 8, 16), z(6, 16, 4)).shape == (0, 16)
+    w16, nowhere = z(6, 16, 8) + 1, z(5, 3, dt=torch.int64) + 6  # every position dropped
+    acts = z(15, 8) + 2
+    out = expert_mlp(z(5, 16) + 1, nowhere, z(5, 3, dt=F32) + 1, z(6, 16, 16) + 1, w16, acts=acts)
+    assert not bool(out.any()) and bool((acts == 2).all())
     assert matmul_int8(z(0, 16, dt=torch.int8), z(0, dt=F32), z(8, 16, dt=torch.int8), z(8, dt=F32)).shape == (0, 8)
 
 

@@ -31,7 +31,7 @@ def _int8(L, n=4, ldx=16, S=4, E=1, N=8, K=16, ldw=16, stride_w=128, bias=None, 
 
 
 @pytest.mark.parametrize("kw", [
-    dict(dtype=0), dict(S=-1), dict(S=2 ** 31), dict(E=0), dict(E=1025), dict(N=0), dict(K=12), dict(ldx=12),
+    dict(dtype=0), dict(S=-1), dict(S=2 ** 30 + 1, n=2 ** 31 - 1), dict(E=0), dict(E=1025), dict(N=0), dict(K=12), dict(ldx=12),
     dict(ldx=8), dict(ldw=20), dict(stride_w=4), dict(stride_w=8), dict(glu=1, N=7), dict(ldy=7), dict(engine=2),
     dict(offsets=None), dict(S=5), dict(X=None), dict(W=None), dict(Y=None), dict(X=ctypes.c_void_p(8)),
     dict(rows=P16, n=0), dict(rows=P16, engine=1)])
