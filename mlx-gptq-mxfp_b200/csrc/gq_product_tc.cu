@@ -21,19 +21,23 @@
 // the copy: 262 us with cp.async by six warps into the stages, 284 us with gather4 loads
 // issued by six threads (20 ns each, 32 per stage).
 //
-// What bounds it, on the same product: the loads alone take 135 us (59 bytes per cycle and
-// SM, 32 KB per stage), the MMAs alone 124 us at 1.85 GHz, together 178 us with one
-// accumulation per tile: both use shared memory's bandwidth. cuBLAS takes 178 us.
+// What bounds it, on the same product (7 tiles of 64 k-steps per pair): the loads alone take
+// 135 us (32 KB per step, 109 GB/s per SM). The MMAs are 512 cycles per step by arithmetic,
+// 146 us at the 1.58 GHz that the SMs hold here, and the tensor pipes read active for 76% of
+// the kernel's 188 us. Loads and MMAs share shared memory's bandwidth. The library's product
+// takes 184 us, as this kernel does with one accumulation per tile.
 //
 // Precision: a tensor-core step loses up to a float32 step of the partial sum, always
 // toward zero, so one accumulator over K = 2048 drifts by 5e-6 of |y| (8 x a float32 FMA
 // chain). The 16-bit kinds therefore leave TMEM every kChunk k-steps and add the chunks in
 // registers, rounding to nearest (the same remedy as in gq_hessian.cu): 1024 products, which
-// keeps the drift 30 times below an f16 output's rounding and costs 3%. Before SwiGLU, whose
+// keeps the drift 30 times below an f16 output's rounding and costs 2 to 3%. Before SwiGLU, whose
 // rows are operands again, sums stay as near as an FMA chain's: with L k-steps per chunk the
 // drift is proportional to L |y|, the chain's rounding grows with sqrt(K) at most, so L is 7 at
-// K = 2048 (1.3 x the chain's error, for 12% of the time: a drain of the accumulator takes
-// 0.3 us from the MMAs), grows with sqrt(K) above and shrinks with K below. s32 sums are
+// K = 2048 (error of the SwiGLU rows once rounded to bf16, pooled over 24 inputs: 1.2 x a
+// float32 product's, 3.0 x with one accumulation; as that goes with the root of the float32
+// error, 1.5 x and 9 x of it. 430 us against 397 for 16384 x 2048 x 8192 and 450 against 420 for 128 experts of
+// [1536, 2048] with 65536 rows, both with one accumulation per tile), grows with sqrt(K) above and shrinks with K below. s32 sums are
 // exact: one accumulation per tile.
 // Every wait is bounded (gq_common.cuh); a wait that gives up records GQ_ERR_TIMEOUT.
 #include <algorithm>

@@ -126,12 +126,12 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
 
-_HERE = contextlib.nullcontext()
+_CURRENT = contextlib.nullcontext()
 
 
 def on(device: torch.device):
     """A context in which launches go to `device`, whatever device is current."""
-    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+    return _CURRENT if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
