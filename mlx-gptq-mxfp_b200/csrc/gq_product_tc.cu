@@ -31,14 +31,14 @@
 // toward zero, so one accumulator over K = 2048 drifts by 5e-6 of |y| (8 x a float32 FMA
 // chain). The 16-bit kinds therefore leave TMEM every kChunk k-steps and add the chunks in
 // registers, rounding to nearest (the same remedy as in gq_hessian.cu): 1024 products, which
-// keeps the drift 30 times below an f16 output's rounding and costs 2 to 3%. Before SwiGLU, whose
-// rows are operands again, sums stay as near as an FMA chain's: with L k-steps per chunk the
-// drift is proportional to L |y|, the chain's rounding grows with sqrt(K) at most, so L is 7 at
-// K = 2048 (error of the SwiGLU rows once rounded to bf16, pooled over 24 inputs: 1.2 x a
-// float32 product's, 3.0 x with one accumulation; as that goes with the root of the float32
-// error, 1.5 x and 9 x of it. 430 us against 397 for 16384 x 2048 x 8192 and 450 against 420 for 128 experts of
-// [1536, 2048] with 65536 rows, both with one accumulation per tile), grows with sqrt(K) above and shrinks with K below. s32 sums are
-// exact: one accumulation per tile.
+// keeps the drift 30 times below an f16 output's rounding and costs 2 to 3%. Before SwiGLU,
+// whose rows are operands again, sums stay as near as an FMA chain's: with L k-steps per
+// chunk the drift is proportional to L |y|, the chain's rounding grows with sqrt(K) at most,
+// so L is 7 at K = 2048, grows with sqrt(K) above and shrinks with K below. Measured there:
+// the rows' error, once rounded to bf16, is 1.2 x that of a float32 product's rows, 3.0 x
+// with one accumulation (this goes with the root of the float32 error: 1.5 x and 9 x of it);
+// 430 us against 397 with one for 16384 x 2048 x 8192, 450 against 420 for 65536 rows of 128
+// experts of [1536, 2048]. s32 sums are exact: one accumulation per tile.
 // Every wait is bounded (gq_common.cuh); a wait that gives up records GQ_ERR_TIMEOUT.
 #include <algorithm>
 #include <type_traits>
