@@ -344,8 +344,10 @@ int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, co
  * weights[t, j] * down_e(silu(gate_e x_t) * up_e x_t), e = index[t, j].
  * X: [T, K] of dtype (GQ_BF16 / GQ_F16); gate_up: [E, 2 I, K]; down: [E, N, I];
  * acts: [T * k, I], the rows between the products in slot order (nullable; rows behind the
- * last slot are left alone); out: [T, N]. I, K and the strides multiples of 8. The rows
- * between the products and the rows before the sum are rounded to dtype.
+ * last slot are left alone); out: [T, N]. K and the strides multiples of 8. I a multiple of 8;
+ * any other I goes with acts, and then the columns of acts and down from I up to the next
+ * multiple of 8 are read and have to hold zeros. The rows between the products are rounded to
+ * dtype; the second product's rows are summed in fp32 and only the sum is rounded.
  * own_acts: 1 when acts will be NULL. */
 size_t gq_expert_mlp_workspace_size(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, int64_t N, int own_acts);
 int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, const void* index, int index_bits,

@@ -56,14 +56,14 @@ int run(const char* what, const Args& a, Kind kind, bool glu, int engine, void* 
 // early (see Args): only for launches that follow one of this library's own kernels.
 int grouped(bool early, const void* X, int64_t n, int64_t ldx, const int32_t* rows, int64_t S, const int64_t* offsets,
             int64_t E, const void* W, int64_t N, int64_t K, int64_t ldw, int64_t stride_w, int dtype, int glu, void* Y,
-            int64_t ldy, int zero_behind, int engine, void* workspace, size_t workspace_bytes, int32_t* status,
+            int out_dtype, int64_t ldy, int zero_behind, int engine, void* workspace, size_t workspace_bytes, int32_t* status,
             void* stream) {
   GQ_REQUIRE(dtype == GQ_BF16 || dtype == GQ_F16, "gq_matmul_grouped: rows and weights are bf16 or f16 (dtype %d)",
              dtype);
   Args a = {};
   a.X = (const uint8_t*)X, a.n_src = n, a.ldx = 2 * ldx, a.rows = rows, a.offsets = offsets, a.E = E, a.S = S;
   a.W = (const uint8_t*)W, a.N = N, a.K = K, a.ldw = 2 * ldw, a.stride_w = 2 * stride_w;
-  a.Y = Y, a.ldy = ldy, a.out_dtype = dtype, a.zero_behind = zero_behind, a.status = status, a.early = early;
+  a.Y = Y, a.ldy = ldy, a.out_dtype = out_dtype, a.zero_behind = zero_behind, a.status = status, a.early = early;
   return run("gq_matmul_grouped", a, dtype == GQ_BF16 ? BF16 : F16, glu != 0, engine, workspace, workspace_bytes,
              (cudaStream_t)stream);
 }
@@ -103,8 +103,8 @@ extern "C" int gq_matmul_grouped(const void* X, int64_t n, int64_t ldx, const in
                                  const int64_t* offsets, int64_t E, const void* W, int64_t N, int64_t K, int64_t ldw,
                                  int64_t stride_w, int dtype, int glu, void* Y, int64_t ldy, int zero_behind,
                                  int engine, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-  return prod::grouped(false, X, n, ldx, rows, S, offsets, E, W, N, K, ldw, stride_w, dtype, glu, Y, ldy, zero_behind,
-                       engine, workspace, workspace_bytes, status, stream);
+  return prod::grouped(false, X, n, ldx, rows, S, offsets, E, W, N, K, ldw, stride_w, dtype, glu, Y, dtype, ldy,
+                       zero_behind, engine, workspace, workspace_bytes, status, stream);
 }
 
 extern "C" int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, const int32_t* rows,
@@ -142,7 +142,7 @@ MlpPlan mlp_plan(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, int64_t 
   p.offsets = take(size_t(E + 1) * 8);
   p.route = take(gq_route_slots_workspace_size(T, k, E));
   p.acts = take(own_acts ? S * size_t(I) * 2 : 0);
-  p.y = take(S * size_t(N) * 2);
+  p.y = take(S * size_t(N) * 4);  // float32: the weighted sum takes the products unrounded
   p.gathered = take(gq_matmul_workspace_size(int64_t(S), E, K, 2, -1));
   p.total = at;
   return p;
@@ -164,7 +164,9 @@ extern "C" int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, c
   GQ_REQUIRE(T >= 0 && k >= 1 && T <= INT32_MAX / k && E >= 1 && K >= 1 && I >= 1 && N >= 1, "gq_expert_mlp: sizes");
   if (T == 0) return GQ_OK;
   GQ_REQUIRE(index && weights && out, "gq_expert_mlp: null pointer");
-  GQ_REQUIRE(I % 8 == 0 && (!acts || ld_acts % 8 == 0), "gq_expert_mlp: activation rows must be 16-byte aligned");
+  const int64_t Kd = (I + 7) / 8 * 8;  // what the second product contracts; columns [I, Kd) hold zeros
+  GQ_REQUIRE(acts ? ld_acts % 8 == 0 && ld_acts >= Kd : I % 8 == 0,
+             "gq_expert_mlp: activation rows must be 16-byte aligned and hold I rounded up to 8");
   const MlpPlan p = mlp_plan(T, k, E, K, I, N, acts == nullptr);
   if (prod::token_fits(T, k, E) && (acts || (workspace && workspace_bytes >= p.total && aligned16(workspace)))) {
     prod::Args up = {}, dn = {};
@@ -173,7 +175,7 @@ extern "C" int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, c
     up.W = (const uint8_t*)gate_up, up.N = 2 * I, up.K = K, up.ldw = 2 * ld_gate_up, up.stride_w = 2 * stride_gate_up;
     up.Y = acts, up.ldy = ld_acts, up.out_dtype = dtype;
     dn.X = (const uint8_t*)acts, dn.n_src = k, dn.ldx = 2 * ld_acts, dn.E = E, dn.S = 1, dn.offsets = up.offsets;
-    dn.W = (const uint8_t*)down, dn.N = N, dn.K = I, dn.ldw = 2 * ld_down, dn.stride_w = 2 * stride_down;
+    dn.W = (const uint8_t*)down, dn.N = N, dn.K = Kd, dn.ldw = 2 * ld_down, dn.stride_w = 2 * stride_down;
     dn.Y = out, dn.ldy = N, dn.out_dtype = dtype;  // offsets: only checked for being there
     GQ_REQUIRE(dtype == GQ_BF16 || dtype == GQ_F16, "gq_expert_mlp: rows and weights are bf16 or f16 (dtype %d)", dtype);
     GQ_REQUIRE(index_bits == 32 || index_bits == 64, "gq_expert_mlp: indices have 32 or 64 bits, not %d", index_bits);
@@ -194,10 +196,10 @@ extern "C" int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, c
   st = gq_matmul_grouped(X, T, ldx, tok, S, offsets, E, gate_up, 2 * I, K, ld_gate_up, stride_gate_up, dtype, 1, acts,
                          ld_acts, 0, -1, ws + p.gathered, p.total - p.gathered, status, stream);
   if (st != GQ_OK) return st;
-  st = prod::grouped(true, acts, S, ld_acts, nullptr, S, offsets, E, down, N, I, ld_down, stride_down, dtype, 0, ws + p.y,
-                         N, 0, -1, nullptr, 0, status, stream);
+  st = prod::grouped(true, acts, S, ld_acts, nullptr, S, offsets, E, down, N, Kd, ld_down, stride_down, dtype, 0,
+                     ws + p.y, GQ_F32, N, 0, -1, nullptr, 0, status, stream);
   if (st != GQ_OK) return st;
-  return gq_combine_slots(ws + p.y, dtype, S, N, slot, weights, T, k, N, out, ldo, stream);
+  return slots::combine_rows(ws + p.y, GQ_F32, dtype, S, N, slot, weights, T, k, N, out, ldo, (cudaStream_t)stream);
 }
 
 extern "C" size_t gq_linear_int8_workspace_size(int64_t M, int64_t K) {

@@ -6,6 +6,11 @@
 #include "gq_common.cuh"
 
 namespace gq {
+namespace slots {
+int combine_rows(const void* y, int y_dtype, int dtype, int64_t S, int64_t ldy, const int32_t* slot,
+                 const float* weights, int64_t T, int64_t k, int64_t N, void* out, int64_t ldo, cudaStream_t s);
+}
+
 namespace prod {
 
 // Element kinds of a product: both operands in the kind, sums in fp32 (s32 for S8, exact).

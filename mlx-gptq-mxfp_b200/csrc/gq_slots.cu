@@ -13,7 +13,7 @@
 // depend on the order in which anything runs.
 #include <algorithm>
 
-#include "gq_common.cuh"
+#include "gq_product.cuh"
 
 namespace gq {
 namespace slots {
@@ -139,11 +139,12 @@ __global__ void __launch_bounds__(THREADS)
 
 // out[t, c .. c + V) = sum over positions j of weights[t, j] * y[slot[t, j], c .. c + V),
 // in position order in fp32, rounded once. HBM-bound: k rows in, one out. A thread takes
-// V = 8 channels (16 bytes; V = 1 where sizes or alignment do not allow that) of one token
-// and has up to eight rows in flight.
-template <typename T, int V>
+// V = 8 channels (16 bytes of out; V = 1 where sizes or alignment do not allow that) of one
+// token and has up to eight rows in flight. Y: T, or float for rows that the sum takes
+// unrounded.
+template <typename Y, typename T, int V>
 __global__ void __launch_bounds__(256)
-    combine_kernel(const T* __restrict__ y, int64_t S, int64_t ldy, const int32_t* __restrict__ slot,
+    combine_kernel(const Y* __restrict__ y, int64_t S, int64_t ldy, const int32_t* __restrict__ slot,
                    const float* __restrict__ weights, int64_t tokens, int64_t k, int64_t N, T* __restrict__ out,
                    int64_t ldo) {
   grid_wait();
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
   for (int64_t j0 = 0; j0 < k; j0 += 8) {
-    T rows[8][V];
+    Y rows[8][V];
     float w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -163,17 +164,21 @@ __global__ void __launch_bounds__(256)
       const bool on = s >= 0 && s < S;
       w[j] = on ? weights[t * k + j0 + j] : 0.0f;
       if (V == 8) {
-        uint4 r = make_uint4(0, 0, 0, 0);
-        if (on) r = *reinterpret_cast<const uint4*>(y + int64_t(s) * ldy + c);
-        *reinterpret_cast<uint4*>(rows[j]) = r;
+        constexpr int PER = 16 / int(sizeof(Y));  // elements per load
+#pragma unroll
+        for (int v = 0; v < V; v += PER) {
+          uint4 r = make_uint4(0, 0, 0, 0);
+          if (on) r = *reinterpret_cast<const uint4*>(y + int64_t(s) * ldy + c + v);
+          *reinterpret_cast<uint4*>(rows[j] + v) = r;
+        }
       } else {
-        rows[j][0] = on ? y[int64_t(s) * ldy + c] : from_f32<T>(0.0f);
+        rows[j][0] = on ? y[int64_t(s) * ldy + c] : from_f32<Y>(0.0f);
       }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = fmaf(w[j], to_f32<T>(rows[j][v]), acc[v]);
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(w[j], to_f32<Y>(rows[j][v]), acc[v]);
   }
   T r[V];
 #pragma unroll
@@ -199,14 +204,30 @@ int route(const I* index, int64_t T, int64_t k, int64_t E, int32_t* tok, int32_t
                           chunk, counts, tok, slot, offsets);
 }
 
-template <typename T>
+template <typename Y, typename T>
 int combine(const void* y, int64_t S, int64_t ldy, const int32_t* slot, const float* weights, int64_t tokens,
             int64_t k, int64_t N, void* out, int64_t ldo, cudaStream_t s) {
-  const bool wide = N % 8 == 0 && ldy % 8 == 0 && ldo % 8 == 0 && aligned16(y) && aligned16(out);
+  const bool wide = N % 8 == 0 && ldy * int64_t(sizeof(Y)) % 16 == 0 && ldo % 8 == 0 && aligned16(y) && aligned16(out);
   const int64_t threads = tokens * (wide ? N / 8 : N);
   const unsigned grid = unsigned((threads + 255) / 256);
-  return launch_dependent("combine_kernel", wide ? combine_kernel<T, 8> : combine_kernel<T, 1>, dim3(grid), 256, 0, s,
-                          (const T*)y, S, ldy, slot, weights, tokens, k, N, (T*)out, ldo);
+  return launch_dependent("combine_kernel", wide ? combine_kernel<Y, T, 8> : combine_kernel<Y, T, 1>, dim3(grid), 256,
+                          0, s, (const Y*)y, S, ldy, slot, weights, tokens, k, N, (T*)out, ldo);
+}
+
+// The weighted sum of rows of y_dtype (float32 or dtype) into rows of dtype.
+int combine_rows(const void* y, int y_dtype, int dtype, int64_t S, int64_t ldy, const int32_t* slot,
+                 const float* weights, int64_t T, int64_t k, int64_t N, void* out, int64_t ldo, cudaStream_t s) {
+  GQ_REQUIRE(S >= 0 && T >= 0 && k >= 1 && N >= 1 && T <= INT32_MAX / k && ldy >= N && ldo >= N,
+             "gq_combine_slots: sizes");
+  GQ_REQUIRE(N <= (int64_t(1) << 38) / (T + 1), "gq_combine_slots: %lld tokens x %lld channels", (long long)T,
+             (long long)N);
+  if (T == 0) return GQ_OK;
+  GQ_REQUIRE(slot && weights && out && (y || S == 0), "gq_combine_slots: null pointer");
+  if (y_dtype == GQ_F32)
+    return dtype == GQ_BF16 ? combine<float, __nv_bfloat16>(y, S, ldy, slot, weights, T, k, N, out, ldo, s)
+                            : combine<float, __half>(y, S, ldy, slot, weights, T, k, N, out, ldo, s);
+  return dtype == GQ_BF16 ? combine<__nv_bfloat16, __nv_bfloat16>(y, S, ldy, slot, weights, T, k, N, out, ldo, s)
+                          : combine<__half, __half>(y, S, ldy, slot, weights, T, k, N, out, ldo, s);
 }
 
 }  // namespace slots
@@ -246,13 +267,5 @@ extern "C" int gq_combine_slots(const void* y, int dtype, int64_t S, int64_t ldy
                                 const float* weights, int64_t T, int64_t k, int64_t N, void* out, int64_t ldo,
                                 void* stream) {
   GQ_REQUIRE(dtype == GQ_BF16 || dtype == GQ_F16, "gq_combine_slots: rows are bf16 or f16 (dtype %d)", dtype);
-  GQ_REQUIRE(S >= 0 && T >= 0 && k >= 1 && N >= 1 && T <= INT32_MAX / k && ldy >= N && ldo >= N,
-             "gq_combine_slots: sizes");
-  GQ_REQUIRE(N <= (int64_t(1) << 38) / (T + 1), "gq_combine_slots: %lld tokens x %lld channels", (long long)T,
-             (long long)N);
-  if (T == 0) return GQ_OK;
-  GQ_REQUIRE(slot && weights && out && (y || S == 0), "gq_combine_slots: null pointer");
-  cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == GQ_BF16) return slots::combine<__nv_bfloat16>(y, S, ldy, slot, weights, T, k, N, out, ldo, s);
-  return slots::combine<__half>(y, S, ldy, slot, weights, T, k, N, out, ldo, s);
+  return slots::combine_rows(y, dtype, dtype, S, ldy, slot, weights, T, k, N, out, ldo, (cudaStream_t)stream);
 }

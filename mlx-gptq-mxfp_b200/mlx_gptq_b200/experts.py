@@ -25,7 +25,7 @@ F.linear interception stashes (capture.py:192-207), without per-expert copies.
 (products.py): slots ordered on the device, one product with SwiGLU and one without,
 each slot's row summed per token, no host read unless a CaptureManager is active (one,
 for the counts). It captures the same rows of the same tokens; values are rounded once
-per product and once per token instead of after every elementwise step, so they agree
+before the second product and once per token instead of after every step, so they agree
 with the eager loop's within its roundings, not bit for bit.
 """
 
@@ -167,15 +167,15 @@ def fused_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torch.
     sink = getattr(self, "_gq_sink", None)
     if sink is None:
         return products.expert_mlp(hidden_states, top_k_index, top_k_weights, self.gate_up_proj, self.down_proj)
-    T, I = hidden_states.shape[0], self.down_proj.shape[-1]
-    tok, slot, offsets = products.route_slots(top_k_index, self.gate_up_proj.shape[0])
+    (T, k), I = top_k_index.shape, self.down_proj.shape[-1]
+    tok, _, offsets = products.route_slots(top_k_index, self.gate_up_proj.shape[0])
+    h = sink.acts_out(T * k, T, I, hidden_states.dtype, hidden_states.device)
+    if h is None:
+        h = torch.empty(T * k, I, dtype=hidden_states.dtype, device=hidden_states.device)
+    out = products.expert_mlp(hidden_states, top_k_index, top_k_weights, self.gate_up_proj, self.down_proj, acts=h)
     counts = offsets.diff().tolist()
     S = sum(counts)
-    h = sink.acts_out(S, T, I, hidden_states.dtype, hidden_states.device)
-    h = products.matmul_grouped(hidden_states, self.gate_up_proj, offsets, rows=tok[:S], glu=True, out=h)
-    y = products.matmul_grouped(h, self.down_proj, offsets)
-    out = products.combine_slots(y, slot, top_k_weights)
-    sink(hidden_states, tok[:S], counts, h)
+    sink(hidden_states, tok[:S], counts, h[:S])
     return out
 
 

@@ -8,7 +8,7 @@ Here:
   and the weighted sum of the slots' rows per token;
 * ``matmul_grouped``: rows of every expert times that expert's weights, ragged sizes,
   rows optionally taken through a row list, SwiGLU optionally applied;
-* ``expert_mlp``: the expert MLP of a routed batch from the three above;
+* ``expert_mlp``: the expert MLP of a routed batch from the kernels of the three above;
 * ``matmul_int8`` / ``matmul_grouped_int8`` / ``linear_int8``: the same products on 8-bit
   codes with one scale per row and one per channel (codes from
   ``grid.rtn_quantize_int8``).
@@ -252,9 +252,9 @@ def expert_mlp(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.
     x: bf16 or f16 [T, C]; top_k_index: int32 / int64 [T, k] (an index outside [0, E) adds
     nothing); top_k_weights: float [T, k]; gate_up: [E, 2 I, C] (gate channels, then up);
     down: [E, C', I], in x's type. Products and sums are float32; the rows between the two
-    products and the rows before the sum are rounded to x's type. acts ([T * k, I]): where
-    the rows that feed down are written, in route_slots order (rows behind the last slot
-    are left alone). Returns [T, C']."""
+    products are rounded to x's type, the second product's rows are summed unrounded and
+    their sum is rounded once. acts ([T * k, I]): where the rows that feed down are written,
+    in route_slots order (rows behind the last slot are left alone). Returns [T, C']."""
     dev = _forward_only("expert_mlp", x, top_k_index, top_k_weights, gate_up, down, acts, out)
     _check_pair(x, gate_up, 3)
     dtype, shape_up, shape_down, shape_idx = x.dtype, gate_up.shape, down.shape, top_k_index.shape
@@ -269,31 +269,32 @@ def expert_mlp(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.
     if dtype not in (torch.bfloat16, torch.float16) or gate_up.dtype != dtype or down.dtype != dtype:
         raise ValueError(f"rows and weights must all be bf16 or f16, not {dtype}, {gate_up.dtype} and {down.dtype}")
     (T, k), (E, N, I) = shape_idx, shape_down
-    ld_acts = 0
     if acts is not None:
         acts = _output(acts, (T * k, I), dtype, dev, "acts")
-        ld_acts = _ld(acts)
     out = _output(out, (T, N), dtype, dev)
     if T == 0:
         return out
+    h, ld_acts = acts, 0 if acts is None else _ld(acts)
     if I % 8 or (acts is not None and (ld_acts % 8 or acts.data_ptr() % 16)):
-        # activation rows that the second product cannot read in place
-        tok, slot, offsets = route_slots(top_k_index, E)
-        h = matmul_grouped(x, gate_up, offsets, rows=tok, glu=True, out=acts)
-        y = matmul_grouped(h, down, offsets)
-        return combine_slots(y, slot, top_k_weights, out=out)
+        # rows that the second product cannot read in place: padded ones, zeros behind column I
+        ld_acts = -(-I // 8) * 8
+        h = torch.zeros(T * k, ld_acts, dtype=dtype, device=dev)
+        if acts is not None:
+            h[:, :I] = acts  # for the rows behind the last slot
     xo, ldx, _ = _operand(x)
     gu, ld_gu, stride_gu = _operand(gate_up)
     dn, ld_dn, stride_dn = _operand(down)
     idx, wt = top_k_index.contiguous(), _weights(top_k_weights)
     K = gu.shape[2]
-    nbytes = _size("gq_expert_mlp_workspace_size", T, k, E, K, I, N, int(acts is None))
+    nbytes = _size("gq_expert_mlp_workspace_size", T, k, E, K, I, N, int(h is None))
     ws = _scratch(nbytes, dev)
     with _on(dev):
         L.check(L.lib().gq_expert_mlp(
             xo.data_ptr(), L.DTYPE_CODE[dtype], T, ldx, idx.data_ptr(), _INDEX_BITS[idx.dtype], wt.data_ptr(), k,
-            gu.data_ptr(), ld_gu, stride_gu, dn.data_ptr(), ld_dn, stride_dn, E, K, I, N, L.ptr(acts), ld_acts,
+            gu.data_ptr(), ld_gu, stride_gu, dn.data_ptr(), ld_dn, stride_dn, E, K, I, N, L.ptr(h), ld_acts,
             out.data_ptr(), _ld(out), L.ptr(ws), nbytes, _status(dev), _stream(dev)), "expert_mlp")
+    if acts is not None and h is not acts:
+        acts.copy_(h[:, :I])
     return out
 
 
