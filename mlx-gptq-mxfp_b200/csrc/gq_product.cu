@@ -1,6 +1,8 @@
 // C entry points of the products of activation rows with weights: argument checks and the
 // choice between the few-rows kernel (gq_product_rows.cu) and the tcgen05 kernel
 // (gq_product_tc.cu).
+#include <algorithm>
+
 #include "gq_product.cuh"
 
 namespace gq {
@@ -125,7 +127,7 @@ namespace {
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct MlpPlan {
-  size_t tok, slot, offsets, route, acts, y, gathered, total;
+  size_t tok, slot, offsets, route, acts, y, gathered, gathered_bytes, total;
 };
 
 MlpPlan mlp_plan(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, int64_t N, bool own_acts) {
@@ -142,8 +144,11 @@ MlpPlan mlp_plan(int64_t T, int64_t k, int64_t E, int64_t K, int64_t I, int64_t 
   p.offsets = take(size_t(E + 1) * 8);
   p.route = take(gq_route_slots_workspace_size(T, k, E));
   p.acts = take(own_acts ? S * size_t(I) * 2 : 0);
-  p.y = take(S * size_t(N) * 4);  // float32: the weighted sum takes the products unrounded
-  p.gathered = take(gq_matmul_workspace_size(int64_t(S), E, K, 2, -1));
+  // The gathered rows and the second product's rows share their bytes: the first product has
+  // read the one when the second writes the other, which it does behind grid_wait(). y is
+  // float32: the weighted sum takes the products unrounded.
+  p.gathered_bytes = gq_matmul_workspace_size(int64_t(S), E, K, 2, -1);
+  p.gathered = p.y = take(std::max(S * size_t(N) * 4, p.gathered_bytes));
   p.total = at;
   return p;
 }
@@ -194,7 +199,7 @@ extern "C" int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, c
   int st = gq_route_slots(index, index_bits, T, k, E, tok, slot, offsets, ws + p.route, p.acts - p.route, stream);
   if (st != GQ_OK) return st;
   st = gq_matmul_grouped(X, T, ldx, tok, S, offsets, E, gate_up, 2 * I, K, ld_gate_up, stride_gate_up, dtype, 1, acts,
-                         ld_acts, 0, -1, ws + p.gathered, p.total - p.gathered, status, stream);
+                         ld_acts, 0, -1, ws + p.gathered, p.gathered_bytes, status, stream);
   if (st != GQ_OK) return st;
   st = prod::grouped(true, acts, S, ld_acts, nullptr, S, offsets, E, down, N, Kd, ld_down, stride_down, dtype, 0,
                      ws + p.y, GQ_F32, N, 0, -1, nullptr, 0, status, stream);
