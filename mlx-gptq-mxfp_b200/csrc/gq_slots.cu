@@ -198,8 +198,11 @@ int route(const I* index, int64_t T, int64_t k, int64_t E, int32_t* tok, int32_t
                                     int(E), chunk, counts);
     if (st != GQ_OK) return st;
   }
-  const size_t smem = size_t(WARPS) * size_t(E + 1) * 2;  // up to 64 KB + 64
-  GQ_CUDA_TRY(cudaFuncSetAttribute(place_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  // The limit is one value per function and device, shared by every host thread: always the
+  // largest, whatever this call needs of it.
+  constexpr size_t most = size_t(WARPS) * size_t(kMaxExperts + 1) * 2;  // 64 KB + 64
+  const size_t smem = size_t(WARPS) * size_t(E + 1) * 2;
+  GQ_CUDA_TRY(cudaFuncSetAttribute(place_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most)));
   return launch_dependent("place_kernel", place_kernel<I>, dim3(unsigned(n)), THREADS, smem, s, index, T, k, int(E),
                           chunk, counts, tok, slot, offsets);
 }
