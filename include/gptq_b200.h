@@ -332,7 +332,7 @@ int gq_matmul_grouped(const void* X, int64_t n, int64_t ldx, const int32_t* rows
 /* The same for 8-bit codes: z = (Xq Wq^T, exact 32-bit sums) * xs[row] * ws[e, channel]
  * (+ bias[channel], dense only: offsets NULL, no glu) in fp32, rounded once to out_dtype
  * (GQ_BF16 / GQ_F16 / GQ_F32). xs: fp32 [n]; ws: fp32 [E, N]; K, ldx, ldw, stride_w
- * multiples of 16, K <= 131071. */
+ * multiples of 16, K <= 131056. */
 int gq_matmul_int8(const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, const int32_t* rows, int64_t S,
                    const int64_t* offsets, int64_t E, const int8_t* Wq, const float* ws, int64_t N, int64_t K,
                    int64_t ldw, int64_t stride_w, const void* bias, int bias_dtype, int glu, void* Y, int out_dtype,
@@ -357,7 +357,8 @@ int gq_expert_mlp(const void* X, int dtype, int64_t T, int64_t ldx, const void* 
                   int32_t* status, void* stream);
 
 /* A linear layer in 8 bits in one call: gq_rtn_int8 on the rows of X [M, K], then
- * gq_matmul_int8 with Wq (codes [N, K rounded up to 16], zeros behind K) and ws [N]. */
+ * gq_matmul_int8 with Wq (codes [N, K rounded up to 16], zeros behind K) and ws [N].
+ * K <= 131056. */
 size_t gq_linear_int8_workspace_size(int64_t M, int64_t K);
 int gq_linear_int8(const void* X, int dtype, int64_t M, int64_t K, int64_t ldx, const int8_t* Wq, const float* ws,
                    int64_t N, int64_t ldw, const void* bias, int bias_dtype, void* Y, int out_dtype, int64_t ldy,

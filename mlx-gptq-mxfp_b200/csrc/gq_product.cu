@@ -79,8 +79,8 @@ int int8(bool early, const int8_t* Xq, const float* xs, int64_t n, int64_t ldx, 
   GQ_REQUIRE(!bias || bias_dtype == GQ_BF16 || bias_dtype == GQ_F16 || bias_dtype == GQ_F32,
              "gq_matmul_int8: bias dtype %d", bias_dtype);
   GQ_REQUIRE(!bias || (!offsets && !glu), "gq_matmul_int8: a bias goes with the dense product only");
-  // |sum| <= K * 128 * 128 has to fit 31 bits
-  GQ_REQUIRE(K <= 131071, "gq_matmul_int8: K = %lld, at most 131071 (32-bit sums)", (long long)K);
+  // |sum| <= K * 128 * 128 has to fit 31 bits: the largest multiple of 16 below 2^31 / 2^14
+  GQ_REQUIRE(K <= 131056, "gq_matmul_int8: K = %lld, at most 131056 (32-bit sums)", (long long)K);
   GQ_REQUIRE(S <= 0 || (xs && ws), "gq_matmul_int8: null pointer");
   Args a = {};
   a.X = (const uint8_t*)Xq, a.n_src = n, a.ldx = ldx, a.rows = rows, a.offsets = offsets, a.E = E, a.S = S;
@@ -217,6 +217,7 @@ extern "C" int gq_linear_int8(const void* X, int dtype, int64_t M, int64_t K, in
                               int out_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, int32_t* status,
                               void* stream) {
   if (M == 0) return GQ_OK;
+  GQ_REQUIRE(K <= 131056, "gq_linear_int8: K = %lld, at most 131056 (32-bit sums)", (long long)K);
   const size_t need = gq_linear_int8_workspace_size(M, K);
   GQ_REQUIRE(need && workspace && workspace_bytes >= need && aligned16(workspace),
              "gq_linear_int8: workspace too small (%zu < %zu)", workspace_bytes, need);

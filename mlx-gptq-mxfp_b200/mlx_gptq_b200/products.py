@@ -30,6 +30,9 @@ import torch
 from . import _lib as L
 
 MAX_EXPERTS = 1024
+# Sums of K products of at most 128 * 128 fit 31 bits up to K = 131071; the kernels read rows
+# padded to 16 codes, so this is the largest K whose padded rows keep that.
+MAX_K_INT8 = 131056
 ENGINES = {None: -1, "rows": 0, "tcgen05": 1}
 
 
@@ -320,8 +323,8 @@ def _int8(xq, xs, wq, ws, offsets, rows, bias, glu, out_dtype, out, engine, what
         raise ValueError(f"unsupported dtype {out_dtype}")
     N, K = wq.shape[-2:]
     E = wq.shape[0] if grouped else 1
-    if K > 131071:
-        raise ValueError(f"K = {K}: sums of 8-bit products fit 32 bits up to 131071")
+    if K > MAX_K_INT8:
+        raise ValueError(f"K = {K}: rows of 8-bit codes have at most {MAX_K_INT8} (32-bit sums)")
     xs = _scales(xs, xq.shape[:1], "xs")
     ws = _scales(ws, wq.shape[:-1], "ws")
     off = _offsets(offsets, E, dev) if grouped else None
@@ -351,7 +354,7 @@ def matmul_int8(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.
                 bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
                 out: torch.Tensor | None = None, engine: str | None = None) -> torch.Tensor:
     """y = (xq @ wq.T) * xs[:, None] * ws (+ bias): int8 codes xq [M, K] with a float32 scale
-    per row, wq [N, K] with one per channel. The integer sums are exact (K <= 131071);
+    per row, wq [N, K] with one per channel. The integer sums are exact (K <= 131056);
     scales and bias are applied in float32 and rounded once to out_dtype (bf16, f16, f32)."""
     return _int8(xq, xs, wq, ws, None, None, bias, False, out_dtype, out, engine, "matmul_int8")
 
@@ -381,8 +384,8 @@ def linear_int8(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, bias: torch
     if wq.dtype != torch.int8:
         raise ValueError(f"codes must be int8, not {wq.dtype}")
     N, K = wq.shape
-    if K > 131071:
-        raise ValueError(f"K = {K}: sums of 8-bit products fit 32 bits up to 131071")
+    if K > MAX_K_INT8:
+        raise ValueError(f"K = {K}: rows of 8-bit codes have at most {MAX_K_INT8} (32-bit sums)")
     ws = _scales(ws, (N,), "ws")
     if bias is not None:
         bias = _check_bias(bias, N)
