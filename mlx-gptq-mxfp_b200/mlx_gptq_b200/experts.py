@@ -64,11 +64,13 @@ def route(top_k_index: torch.Tensor, num_experts: int):
 
     Returns (tok, pos, counts, counts_dev): token and top-k position of each
     ordered slot (int64, on the device), the per-expert slot counts as a host list
-    and as a device tensor. Slots routed to index num_experts (dropped) are left out."""
+    and as a device tensor. Slots routed to an index outside [0, num_experts) (dropped)
+    are left out."""
     T, k = top_k_index.shape
     dev = top_k_index.device
     E = num_experts
-    e = top_k_index.reshape(-1).long().clamp(0, E)
+    e = top_k_index.reshape(-1).long()
+    e = torch.where((e < 0) | (e > E), E, e)
     j = torch.arange(k, device=dev).repeat(T)
     t = torch.arange(T, device=dev).repeat_interleave(k)
     order = torch.argsort(e * (k * T) + j * T + t)
