@@ -163,8 +163,10 @@ def supports_fused(module: torch.nn.Module) -> bool:
 def fused_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                           top_k_weights: torch.Tensor) -> torch.Tensor:
     """The expert forward on the library's products (bound to the module as `forward`); on
-    host tensors, and in types they do not take, the sort-based forward above."""
-    if not hidden_states.is_cuda or hidden_states.dtype not in (torch.bfloat16, torch.float16):
+    host tensors, and in types they do not take (float32, or rows and weights of two types),
+    the sort-based forward above."""
+    if not hidden_states.is_cuda or hidden_states.dtype not in (torch.bfloat16, torch.float16) or not (
+            self.gate_up_proj.dtype == self.down_proj.dtype == hidden_states.dtype):
         return grouped_experts_forward(self, hidden_states, top_k_index, top_k_weights)
     sink = getattr(self, "_gq_sink", None)
     if sink is None:
