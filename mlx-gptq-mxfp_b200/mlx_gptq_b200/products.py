@@ -15,7 +15,8 @@ Here:
 
 All run on the tensors' CUDA device and its current stream and never wait for the
 device, so they can be captured into a CUDA graph (after one ordinary call per device).
-They have no backward: with gradients enabled, inputs that require them are refused.
+They have no derivatives: with gradients enabled, inputs that require them are refused, and
+so are inputs that carry a forward-mode tangent.
 The tensor-core kernel's waits are bounded like the Hessian's: one that gives up leaves
 GQ_ERR_TIMEOUT in the device's status word, which _lib.raise_on_device_timeout reads (and
 every solver before it uses a Hessian).
@@ -26,6 +27,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -37,12 +39,17 @@ ENGINES = {None: -1, "rows": 0, "tcgen05": 1}
 
 
 def _forward_only(what: str, *tensors) -> torch.device:
-    """The tensors' common CUDA device; refuses a call that autograd would have to follow."""
+    """The tensors' common CUDA device; refuses a call that autograd, backward or forward,
+    would have to follow."""
     dev = L.require_cuda(*tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:  # inside a dual level, which no_grad does not end
+        for t in tensors:
+            if t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward derivative: its inputs must not carry tangents")
     return dev
 
 
