@@ -18,8 +18,9 @@ device, so they can be captured into a CUDA graph (after one ordinary call per d
 They have no derivatives: with gradients enabled, inputs that require them are refused, and
 so are inputs that carry a forward-mode tangent.
 The tensor-core kernel's waits are bounded like the Hessian's: one that gives up leaves
-GQ_ERR_TIMEOUT in the device's status word, which _lib.raise_on_device_timeout reads (and
-every solver before it uses a Hessian).
+GQ_ERR_TIMEOUT in the device's status word and rows unwritten. raise_on_device_timeout, which
+waits for the device, reads the word and raises: call it before results are used for good
+(solvers do before they use a Hessian, sequential.Pipeline.run before it returns).
 """
 
 from __future__ import annotations

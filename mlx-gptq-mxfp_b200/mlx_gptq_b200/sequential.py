@@ -37,6 +37,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from ._lib import raise_on_device_timeout
 from .capture import CaptureManager
 from .experts import install_grouped_experts
 from .pipeline import LayerSolveArgs, solve_layer
@@ -613,5 +614,7 @@ class Pipeline:
             log.info("layer %d done: %d linears + %d experts | rel_err med=%.4f max=%.4f | capture %.1fs "
                      "solve %.1fs reforward %.1fs total %.1fs", li, n_lin, n_exp, st.rel_err_median,
                      st.rel_err_max, st.capture_s, st.solve_s, st.reforward_s, st.total_s)
+        if self.dev0.type == "cuda":  # no solve follows the last forward
+            raise_on_device_timeout(self.dev0)
         log.info("%d layers done in %.1f min", n_layers, (time.time() - t_start) / 60)
         return batches
