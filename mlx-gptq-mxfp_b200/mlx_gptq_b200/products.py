@@ -134,6 +134,12 @@ def _output(out, shape, dtype, dev, name="out") -> torch.Tensor:
     return out
 
 
+def _wrote(t: torch.Tensor | None) -> None:
+    """Tells autograd that a given tensor was changed in place."""
+    if t is not None:
+        torch.autograd.graph.increment_version(t)
+
+
 _INDEX_BITS = {torch.int32: 32, torch.int64: 64}
 
 
@@ -209,13 +215,14 @@ def combine_slots(y: torch.Tensor, slot: torch.Tensor, weights: torch.Tensor,
     (T, k), (S, N) = slot.shape, y.shape
     if (N > 1 and y.stride(1) != 1) or (S > 1 and y.stride(0) < N):
         y = y.contiguous()
-    out = _output(out, (T, N), y.dtype, dev)
+    given, out = out, _output(out, (T, N), y.dtype, dev)
     if T == 0 or N == 0:
         return out
     sl, w = slot.contiguous(), _weights(weights)
     with _on(dev):
         L.check(L.lib().gq_combine_slots(L.ptr(y), L.DTYPE_CODE[y.dtype], S, _ld(y), L.ptr(sl), L.ptr(w), T, k, N,
                                          L.ptr(out), _ld(out), _stream(dev)), "combine_slots")
+    _wrote(given)
     return out
 
 
@@ -252,6 +259,7 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
                                           wo.shape[-1], ldw, stride_w, L.DTYPE_CODE[x.dtype], int(glu), L.ptr(y),
                                           _ld(y), int(out is None), eng, L.ptr(ws), ws_bytes,
                                           _status(dev), _stream(dev)), "matmul_grouped")
+    _wrote(out)
     return y
 
 
@@ -282,7 +290,7 @@ def expert_mlp(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.
     (T, k), (E, N, I) = shape_idx, shape_down
     if acts is not None:
         acts = _output(acts, (T * k, I), dtype, dev, "acts")
-    out = _output(out, (T, N), dtype, dev)
+    given, out = out, _output(out, (T, N), dtype, dev)
     if T == 0:
         return out
     h, ld_acts = acts, 0 if acts is None else _ld(acts)
@@ -304,8 +312,11 @@ def expert_mlp(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.
             xo.data_ptr(), L.DTYPE_CODE[dtype], T, ldx, idx.data_ptr(), _INDEX_BITS[idx.dtype], wt.data_ptr(), k,
             gu.data_ptr(), ld_gu, stride_gu, dn.data_ptr(), ld_dn, stride_dn, E, K, I, N, L.ptr(h), ld_acts,
             out.data_ptr(), _ld(out), L.ptr(ws), nbytes, _status(dev), _stream(dev)), "expert_mlp")
-    if acts is not None and h is not acts:
+    if h is acts:
+        _wrote(acts)
+    elif acts is not None:
         acts.copy_(h[:, :I])
+    _wrote(given)
     return out
 
 
@@ -355,6 +366,7 @@ def _int8(xq, xs, wq, ws, offsets, rows, bias, glu, out_dtype, out, engine, what
                                        0 if bias is None else L.DTYPE_CODE[bias.dtype], int(glu), L.ptr(y),
                                        L.DTYPE_CODE[out_dtype], _ld(y), int(out is None), eng, L.ptr(ws_), ws_bytes,
                                        _status(dev), _stream(dev)), what)
+    _wrote(out)
     return y
 
 

@@ -1,4 +1,4 @@
-"""The products and autograd: no tangent is dropped silently."""
+"""The products and autograd: no tangent is dropped silently, no write in place goes unnoticed."""
 
 import pytest
 import torch
@@ -48,3 +48,34 @@ def test_inputs_with_tangents_are_refused(name):
                 with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no forward derivative"):
                     call(*dual)
     assert torch.equal(call(*args), want)
+
+
+def test_given_outputs_count_as_changed_in_place():
+    """A tensor that autograd saved and a call then wrote: its backward raises, as after any
+    write in place, instead of using the new values."""
+    from mlx_gptq_b200 import combine_slots, expert_mlp, matmul_grouped, matmul_int8
+
+    c = _calls()
+    (x, w), off = c["matmul_grouped"][1], torch.tensor([0, 2, 4], device="cuda")
+    (y, s, cw), mlp, q = c["combine_slots"][1], c["expert_mlp"][1], c["matmul_int8"][1]
+    odd = torch.ones(2, 10, 16, dtype=BF16, device="cuda"), torch.ones(2, 16, 5, dtype=BF16, device="cuda")
+    writes = [
+        ((4, 8), lambda out: matmul_grouped(x, w, off, out=out)),
+        ((2, 8), lambda out: combine_slots(y, s, cw, out=out)),
+        ((4, 16), lambda out: expert_mlp(*mlp, out=out)),
+        ((8, 8), lambda out: expert_mlp(*mlp, acts=out)),
+        ((8, 5), lambda out: expert_mlp(*mlp[:3], *odd, acts=out)),
+        ((4, 8), lambda out: matmul_int8(*q[:4], out=out)),
+    ]
+    for i, (shape, write) in enumerate(writes):
+        out = torch.ones(shape, dtype=BF16, device="cuda")
+        leaf = torch.ones(shape, dtype=BF16, device="cuda", requires_grad=True)
+        loss = (leaf * out).sum()  # saves out
+        with torch.no_grad():
+            write(out)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            loss.backward()
+            pytest.fail(f"write {i} went unnoticed")
+    with torch.inference_mode():  # tensors without a version
+        out = torch.empty(4, 8, dtype=BF16, device="cuda")
+        assert matmul_grouped(x, w, off, out=out) is out
