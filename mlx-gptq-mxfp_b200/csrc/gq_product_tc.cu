@@ -269,6 +269,14 @@ __device__ __forceinline__ void store_block(const Args& a, int64_t row0, int64_t
       if (j < left) *reinterpret_cast<uint32_t*>(p) = w;
       p += step;
     }
+  } else if (DT == GQ_F32) {
+    float* p = reinterpret_cast<float*>(a.Y) + row0 * a.ldy + ch;
+    const int left = ch < I ? rows : 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (j < left) *p = v[j];
+      p += a.ldy;
+    }
   } else if (ch < I) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)

@@ -139,9 +139,9 @@ __global__ void __launch_bounds__(THREADS)
 
 // out[t, c .. c + V) = sum over positions j of weights[t, j] * y[slot[t, j], c .. c + V),
 // in position order in fp32, rounded once. HBM-bound: k rows in, one out. A thread takes
-// V = 8 channels (16 bytes of out; V = 1 where sizes or alignment do not allow that) of one
-// token and has up to eight rows in flight. Y: T, or float for rows that the sum takes
-// unrounded.
+// the V channels of one token that 16 bytes of a row hold (V = 1 where sizes or alignment do
+// not allow that) and has up to eight rows in flight. Y: T, or float for rows that the sum
+// takes unrounded.
 template <typename Y, typename T, int V>
 __global__ void __launch_bounds__(256)
     combine_kernel(const Y* __restrict__ y, int64_t S, int64_t ldy, const int32_t* __restrict__ slot,
@@ -163,14 +163,10 @@ __global__ void __launch_bounds__(256)
       const int32_t s = j0 + j < k ? slot[t * k + j0 + j] : -1;
       const bool on = s >= 0 && s < S;
       w[j] = on ? weights[t * k + j0 + j] : 0.0f;
-      if (V == 8) {
-        constexpr int PER = 16 / int(sizeof(Y));  // elements per load
-#pragma unroll
-        for (int v = 0; v < V; v += PER) {
-          uint4 r = make_uint4(0, 0, 0, 0);
-          if (on) r = *reinterpret_cast<const uint4*>(y + int64_t(s) * ldy + c + v);
-          *reinterpret_cast<uint4*>(rows[j] + v) = r;
-        }
+      if (V > 1) {  // one 16-byte load of the row
+        uint4 r = make_uint4(0, 0, 0, 0);
+        if (on) r = *reinterpret_cast<const uint4*>(y + int64_t(s) * ldy + c);
+        *reinterpret_cast<uint4*>(rows[j]) = r;
       } else {
         rows[j][0] = on ? y[int64_t(s) * ldy + c] : from_f32<Y>(0.0f);
       }
@@ -185,6 +181,8 @@ __global__ void __launch_bounds__(256)
   for (int v = 0; v < V; ++v) r[v] = from_f32<T>(acc[v]);
   if (V == 8)
     *reinterpret_cast<uint4*>(out + t * ldo + c) = *reinterpret_cast<const uint4*>(r);
+  else if (V == 4)
+    *reinterpret_cast<uint2*>(out + t * ldo + c) = *reinterpret_cast<const uint2*>(r);
   else
     out[t * ldo + c] = r[0];
 }
@@ -210,10 +208,12 @@ int route(const I* index, int64_t T, int64_t k, int64_t E, int32_t* tok, int32_t
 template <typename Y, typename T>
 int combine(const void* y, int64_t S, int64_t ldy, const int32_t* slot, const float* weights, int64_t tokens,
             int64_t k, int64_t N, void* out, int64_t ldo, cudaStream_t s) {
-  const bool wide = N % 8 == 0 && ldy * int64_t(sizeof(Y)) % 16 == 0 && ldo % 8 == 0 && aligned16(y) && aligned16(out);
-  const int64_t threads = tokens * (wide ? N / 8 : N);
+  constexpr int V = 16 / int(sizeof(Y));
+  const bool wide = N % V == 0 && ldy % V == 0 && ldo % V == 0 && aligned16(y) &&
+                    (reinterpret_cast<uintptr_t>(out) & (V * sizeof(T) - 1)) == 0;
+  const int64_t threads = tokens * (wide ? N / V : N);
   const unsigned grid = unsigned((threads + 255) / 256);
-  return launch_dependent("combine_kernel", wide ? combine_kernel<Y, T, 8> : combine_kernel<Y, T, 1>, dim3(grid), 256,
+  return launch_dependent("combine_kernel", wide ? combine_kernel<Y, T, V> : combine_kernel<Y, T, 1>, dim3(grid), 256,
                           0, s, (const Y*)y, S, ldy, slot, weights, tokens, k, N, (T*)out, ldo);
 }
 
