@@ -14,7 +14,10 @@ namespace {
 // rows but has only CTA pairs x 256 channels to spread them over. Measured, 128 experts of
 // [1536, 2048] with SwiGLU and of [2048, 768], both: 64 rows 61 against 66 us, 128 rows 85
 // against 78, 512 rows 191 against 112; dense s8 [4096, 4096], 64 rows 13 against 16 us,
-// 128 rows 23 against 16.
+// 128 rows 23 against 16. The rule fits 128 experts and one. Between them it goes to the
+// tcgen05 kernel too early: evenly routed rows through E experts of [1536, 2048] with SwiGLU,
+// weights from HBM, E = 2 and 8 rows 6 against 16 us, E = 8 and 16 rows 12 against 18, E = 32
+// and 64 rows 29 against 35; the two meet near 128 rows (E = 2 to 8) and 256 (E = 16, 32).
 bool by_rows(int64_t S, int64_t E, int engine) {
   return engine == 0 || (engine < 0 && S <= (E == 1 ? 64 : (E + 1) / 2));
 }

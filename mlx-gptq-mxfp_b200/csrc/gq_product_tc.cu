@@ -16,16 +16,19 @@
 //   warps 0, 2   TMA: weights [expert, channel, k]; rows of X
 //   warp 1       MMA issuer (even CTA) into one of two TMEM accumulator sets
 //   warps 4-11   drain the other set into registers; scale / bias / SwiGLU, round once, store
-// A row list is applied by a copy before the launch (gather_kernel). Gathering inside the
-// kernel was built and measured on 8192 x 4096 x 4096 bf16, 184 us without and 204 us with
-// the copy: 262 us with cp.async by six warps into the stages, 284 us with gather4 loads
-// issued by six threads (20 ns each, 32 per stage).
+// A row list is applied by a copy before the launch (gather_kernel): 8192 x 4096 x 4096 bf16
+// takes 186 us without and 205 us with it. Gathering inside the kernel was built and measured
+// on the same product: 262 us with cp.async by six warps into the stages, 284 us with gather4
+// loads issued by six threads (20 ns each, 32 per stage).
 //
 // What bounds it, on the same product (7 tiles of 64 k-steps per pair): the loads alone take
 // 135 us (32 KB per step, 109 GB/s per SM). The MMAs are 512 cycles per step by arithmetic,
 // 146 us at the 1.58 GHz that the SMs hold here, and the tensor pipes read active for 76% of
-// the kernel's 188 us. Loads and MMAs share shared memory's bandwidth. The library's product
-// takes 184 us, as this kernel does with one accumulation per tile.
+// the kernel's time (188 us under ncu). Loads and MMAs share shared memory's bandwidth. The
+// library's product takes 180 us. Grouped batches stay further from it (65536 rows of 128
+// experts of [1536, 2048], SwiGLU: 422 us, pipes active 47%): uneven experts account for 47
+// us, SwiGLU with its shorter accumulations for 32. Weights from HBM cost at most 39: experts
+// that overlap in memory, and so stay in L2, take 383 us, and equal experts gain nothing by it.
 //
 // Precision: a tensor-core step loses up to a float32 step of the partial sum, always
 // toward zero, so one accumulator over K = 2048 drifts by 5e-6 of |y| (8 x a float32 FMA
